@@ -1,0 +1,503 @@
+"""Measured calls of four operators: storing a prefix's keys and values in a paged 4-bit
+cache (and reading it back), joint attention over that cache, moving its pages, and the
+low-rank adapters of many requests beside a shared projection.
+
+`run` computes them in their plain form (elementary torch operations, 32-bit), or with
+`own` set through b200attn.  The plain form below is also the definition of the cache's
+bytes: a page holds 64 tokens, and one head's part of a page is a block of 9216 bytes,
+
+    [0, 4096)      K numbers    8 token octets x 32 x 16 bytes
+    [4096, 8192)   V numbers    8 token octets x 32 x 16 bytes
+    [8192, 8704)   K steps      8 token octets x 4 x 4 x 2 bf16
+    [8704, 9216)   V steps      the same
+
+A value is step * (nibble - 8), one step for 32 neighbouring channels of one token.
+"""
+import math
+import os
+import random
+import sys
+
+import torch
+
+own = False  # set by the tool: False = plain form, True = the framework's calls
+
+PAGE = 64            # tokens of a page
+BLOCK = 9216         # bytes of one head's part of a page
+D = 128              # head width
+TINY = 2.0 ** -100   # a group whose largest magnitude is below this is stored as zeros
+
+
+def _api():
+    root = os.path.join(os.getcwd(), "qwen3-image21_b200")
+    if root not in sys.path:
+        sys.path.insert(0, root)
+    import b200attn
+    return b200attn
+
+
+# ------------------------------------------------------------------------------ cases
+def listed():
+    return [
+        # One text token appended to a 512-token prefix: one query, latency alone.
+        dict(name="attend_token", op="attend", batch=1, heads=32, tokens=1, prefix=512,
+             causal=False, ragged=False),
+        # Single tokens of 16 requests over prefixes as long as the edit workload's.
+        dict(name="attend_tokens_long", op="attend", batch=16, heads=32, tokens=1, prefix=10587,
+             causal=False, ragged=True),
+        # A few words appended to each of 8 prompts: causal among themselves, ragged.
+        dict(name="attend_extend", op="attend", batch=8, heads=32, tokens=37, prefix=1000,
+             causal=True, ragged=True),
+        # The 1024x1024 denoising step: 4096 image tokens over a 512-token prefix.
+        dict(name="attend_image", op="attend", batch=1, heads=32, tokens=4096, prefix=512,
+             causal=False, ragged=False),
+        # The image-edit step: the prefix holds two condition images (37 keys padded).
+        dict(name="attend_edit", op="attend", batch=1, heads=32, tokens=4096, prefix=10587,
+             causal=False, ragged=False),
+        # Text prefixes of 16 sequences (8 prompts and their negatives), then read whole.
+        dict(name="store_prompts", op="store", batch=16, heads=32, tokens=512, start=0,
+             ragged=True),
+        # 29 more tokens behind what 4 long prefixes hold, in the middle of a page.
+        dict(name="store_extend", op="store", batch=4, heads=32, tokens=29, start=5003,
+             ragged=True),
+        # One request forked: its unfinished last page, in the 32 layers.
+        dict(name="pages_fork", op="pages", layers=32, pages=16, heads=32, moves=1),
+        # A pool made dense after half of its requests left.
+        dict(name="pages_compact", op="pages", layers=16, pages=256, heads=32, moves=120),
+        # One row of each of 4 requests with adapters of their own.
+        dict(name="lora_rows", op="lora", segments=4, rows=4, k=4096, n=4096, rank=16,
+             adapters=4, ragged=False),
+        # 16 prompts' ragged text rows, some requests without an adapter.
+        dict(name="lora_prompts", op="lora", segments=16, rows=4600, k=4096, n=4096, rank=32,
+             adapters=6, ragged=True),
+        # The MLP's first product of 4 images of 1024x1024, adapters of their own.
+        dict(name="lora_images", op="lora", segments=4, rows=16384, k=4096, n=12288, rank=64,
+             adapters=4, ragged=False),
+    ]
+
+
+def _log(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    most = 32 * 4096 * (10587 + 4096)
+    while True:
+        op = rng.choice(("attend", "attend", "attend", "store", "pages", "lora", "lora"))
+        if op == "attend":
+            tokens = _log(rng, 1, 4096) if rng.random() < 0.7 else rng.randint(1, 20)
+            c = dict(op=op, batch=_log(rng, 1, 16), heads=rng.choice((1, 2, 3, 8, 16, 24, 32)),
+                     tokens=tokens, prefix=_log(rng, 1, 10624), causal=rng.random() < 0.4,
+                     ragged=rng.random() < 0.6)
+            if c["batch"] * c["heads"] * tokens * (tokens + c["prefix"]) <= most and \
+                    c["batch"] * c["heads"] * (tokens + c["prefix"]) <= 16 * 32 * 10588:
+                return c
+        elif op == "store":
+            c = dict(op=op, batch=_log(rng, 1, 16), heads=rng.choice((1, 2, 3, 8, 16, 24, 32)),
+                     tokens=_log(rng, 1, 4096), start=rng.choice((0, _log(rng, 1, 6000))),
+                     ragged=rng.random() < 0.6)
+            if c["batch"] * c["heads"] * (c["tokens"] + c["start"]) <= 4 * 32 * 5032:
+                return c
+        elif op == "pages":
+            pages = _log(rng, 4, 256)
+            c = dict(op=op, layers=rng.randint(1, 32), pages=pages, heads=rng.choice((1, 4, 8, 32)),
+                     moves=rng.randint(1, pages // 2))
+            if c["layers"] * pages * c["heads"] <= 16 * 256 * 32 and \
+                    c["layers"] * c["moves"] * c["heads"] <= 16 * 120 * 32:
+                return c
+        else:
+            segments = _log(rng, 1, 48)
+            c = dict(op=op, segments=segments, rows=max(segments, _log(rng, 1, 16384)),
+                     k=8 * rng.randint(8, 1024), n=8 * rng.randint(4, 1536),
+                     rank=rng.choice((8, 16, 24, 32, 64, 128)), adapters=rng.randint(1, 8),
+                     ragged=rng.random() < 0.6)
+            if c["rows"] * (c["k"] + 2 * c["n"]) <= 16384 * (4096 + 2 * 12288) and \
+                    c["segments"] * c["rows"] * (c["k"] + c["n"]) <= 16384 * 16384 * 4:
+                return c
+
+
+# ------------------------------------------------------------- lengths that a case stands for
+def _spread(case, count, most, zero):
+    """Ragged lengths up to `most`, the first one whole; the second may be nothing."""
+    rng = random.Random("%d %d %d" % (count, most, case.get("heads", case.get("k", 0))))
+    got = [max(1, _log(rng, max(1, most // 8), most)) for _ in range(count)]
+    got[0] = most
+    if zero and count > 2:
+        got[1] = 0
+    return got
+
+
+def _prefixes(case):
+    if case["ragged"]:
+        return _spread(case, case["batch"], case["prefix"], True)
+    return [case["prefix"]] * case["batch"]
+
+
+def _targets(case):
+    """Valid tokens of each batch row's own: a padded batch has fewer."""
+    t = case["tokens"]
+    return [max(1, t - 3 * (b % 3)) if case["ragged"] else t for b in range(case["batch"])]
+
+
+def _seen(case, b):
+    """Key and query pairs that batch row b computes."""
+    t, v, p = case["tokens"], _targets(case)[b], _prefixes(case)[b]
+    if case["causal"]:
+        return t * p + sum(min(i + 1, v) for i in range(t))
+    return t * (p + v)
+
+
+def _rows(case):
+    """Rows of each request (they sum to case["rows"])."""
+    s, r = case["segments"], case["rows"]
+    if not case["ragged"]:
+        return [r // s + (1 if i < r % s else 0) for i in range(s)]
+    rng = random.Random("%d %d %d" % (s, r, case["k"]))
+    cuts = sorted(rng.randint(0, r) for _ in range(s - 1))
+    return [b - a for a, b in zip([0] + cuts, cuts + [r])]
+
+
+def _who(case):
+    """Adapter of each request, -1 for none."""
+    s = case["segments"]
+    return [-1 if case["ragged"] and i % 5 == 3 else (i * 7 + 1) % case["adapters"] for i in range(s)]
+
+
+def work(case):
+    if case["op"] == "attend":
+        b, h, t = case["batch"], case["heads"], case["tokens"]
+        pairs = sum(_seen(case, i) for i in range(b))
+        return {"bytes": h * (sum(_prefixes(case)) * BLOCK // PAGE + 4 * b * t * D * 2),
+                "flops": 4 * h * D * pairs}
+    if case["op"] == "store":
+        new = sum(_counts(case)) * case["heads"]
+        total = sum(a + n for a, n in zip(_starts(case), _counts(case))) * case["heads"]
+        return {"bytes": new * (2 * D * 2 + BLOCK // PAGE) + total * 2 * D * 2, "flops": 0}
+    if case["op"] == "pages":
+        return {"bytes": 2 * case["layers"] * case["moves"] * case["heads"] * BLOCK, "flops": 0}
+    rows = sum(n for n, a in zip(_rows(case), _who(case)) if a >= 0)
+    used = len({a for n, a in zip(_rows(case), _who(case)) if a >= 0 and n})
+    k, n, r = case["k"], case["n"], case["rank"]
+    return {"bytes": 2 * (rows * k + 2 * case["rows"] * n + used * r * (k + n)),
+            "flops": 2 * rows * r * (k + n)}
+
+
+def _starts(case):
+    if case["ragged"] and case["start"]:
+        return _spread(case, case["batch"], case["start"], True)
+    return [case["start"]] * case["batch"]
+
+
+def _counts(case):
+    if case["ragged"]:
+        return _spread(case, case["batch"], case["tokens"], False)
+    return [case["tokens"]] * case["batch"]
+
+
+# --------------------------------------------------------------- the cache's bytes, plain form
+def _quantise(x):
+    """x [..., 128] -> numbers uint8 [..., 128] (1..15) and steps f32 [..., 4].  The step is
+    the group's largest magnitude / 7 rounded to 5 significant bits, so that every product
+    step * (number - 8) is a bf16 value; halves round away from zero."""
+    g = x.float().unflatten(-1, (4, 32))
+    top = g.abs().amax(-1)
+    seven = torch.full_like(top, 7.0)  # a tensor: a true division, rounded once
+    bits = (top / seven).view(torch.int32)
+    step = (((bits + 0x3FFFF + ((bits >> 19) & 1)) >> 19) << 19).view(torch.float32)
+    step = torch.where(top < TINY, torch.zeros_like(step), step)
+    step = torch.where(torch.isfinite(top), step, torch.full_like(step, math.nan))
+    use = (step > 0).unsqueeze(-1)
+    mag = torch.floor(g.abs() / torch.where(use, step.unsqueeze(-1), 1.0) + 0.5)
+    num = torch.where(use, torch.sign(g) * mag, 0.0)
+    return (num + 8).to(torch.uint8).flatten(-2), step
+
+
+def _pack(kn, ks, vn, vs):
+    """Numbers uint8 [..., 64, 128] and steps f32 [..., 64, 4] of K and V -> blocks uint8
+    [..., 9216]."""
+    lead = kn.shape[:-2]
+    # K: token = 8 a + g, channel = 32 c + 8 t + j; stored by (a, g, t, c, j)
+    k = kn.unflatten(-2, (8, 8)).unflatten(-1, (4, 4, 8)).transpose(-2, -3)
+    # V: token = 8 a + 2 t + p, channel = 32 c + 4 g + i; stored by (a, g, t, c, p, i)
+    v = vn.unflatten(-2, (8, 4, 2)).unflatten(-1, (4, 8, 4))
+    n = len(lead)
+    v = v.permute(*range(n), n, n + 4, n + 1, n + 3, n + 2, n + 5)  # a t p c g i -> a g t c p i
+
+    def nibbles(z):
+        z = z.reshape(*lead, 4096, 2)
+        return z[..., 0] | (z[..., 1] << 4)
+
+    def steps(z):  # token = 8 a + 2 t + p; stored by (a, t, c, p)
+        z = z.to(torch.bfloat16).unflatten(-2, (8, 4, 2)).transpose(-1, -2).contiguous()
+        return z.view(torch.uint8).reshape(*lead, 512)
+
+    return torch.cat([nibbles(k), nibbles(v), steps(ks), steps(vs)], -1)
+
+
+def _unpack(blocks):
+    """The inverse of _pack: blocks uint8 [..., 9216] -> kn, ks, vn, vs."""
+    lead = blocks.shape[:-1]
+    n = len(lead)
+
+    def nibbles(z):
+        return torch.stack([z & 15, z >> 4], -1).reshape(*lead, -1)
+
+    k = nibbles(blocks[..., :4096]).view(*lead, 8, 8, 4, 4, 8).transpose(-2, -3)
+    v = nibbles(blocks[..., 4096:8192]).view(*lead, 8, 8, 4, 4, 2, 4)
+    v = v.permute(*range(n), n, n + 2, n + 4, n + 3, n + 1, n + 5)  # a g t c p i -> a t p c g i
+
+    def steps(z):
+        z = z.contiguous().view(torch.bfloat16).float().view(*lead, 8, 4, 4, 2)
+        return z.transpose(-1, -2).reshape(*lead, 64, 4)
+
+    return (k.reshape(*lead, 64, 128), steps(blocks[..., 8192:8704]),
+            v.reshape(*lead, 64, 128), steps(blocks[..., 8704:9216]))
+
+
+def _values(num, step):
+    return ((num.float() - 8.0).unflatten(-1, (4, 32)) * step.unsqueeze(-1)).flatten(-2)
+
+
+def _gather(pool, table):
+    """pool [pages, H, 9216], table int32 [B, M] -> blocks [B, H, M, 9216]."""
+    return pool[table.clamp(min=0).long()].transpose(1, 2)
+
+
+def _rows_of(z):
+    """[B, H, M, 64, W] -> [B, H, M * 64, W]"""
+    return z.flatten(2, 3)
+
+
+# ----------------------------------------------------------------------------------- prepare
+def _pages_for(lengths, gen, device):
+    """A pool's size and a page table for sequences of these lengths: pages in random order,
+    a few pages unused, -1 behind each row's last page."""
+    need = [(n + PAGE - 1) // PAGE for n in lengths]
+    total = sum(need) + 3
+    order = torch.randperm(total, generator=gen, device=device).to(torch.int32)
+    table = torch.full((len(lengths), max(1, max(need))), -1, dtype=torch.int32, device=device)
+    at = 0
+    for b, n in enumerate(need):
+        table[b, :n] = order[at:at + n]
+        at += n
+    return total, table
+
+
+def _filled_pool(lengths, heads, gen, device, extra=None):
+    """A pool that holds N(0, 1) keys and values of these lengths; every byte that no token
+    owns is random.  `extra`: the lengths that the page table has room for."""
+    room = lengths if extra is None else extra
+    total, table = _pages_for(room, gen, device)
+    pool = torch.randint(0, 256, (total, heads, BLOCK), generator=gen, device=device, dtype=torch.uint8)
+    for b, n in enumerate(lengths):  # sequence by sequence: the 32-bit values stay small
+        m = (n + PAGE - 1) // PAGE
+        if m == 0:
+            continue
+        ids = table[b, :m].long()
+        kn, ks, vn, vs = _unpack(pool[ids])
+        fresh = [_quantise(torch.randn(m, heads, PAGE, D, generator=gen, device=device).bfloat16())
+                 for _ in range(2)]
+        live = (torch.arange(m * PAGE, device=device) < n).view(m, 1, PAGE, 1)
+        pool[ids] = _pack(torch.where(live, fresh[0][0], kn), torch.where(live, fresh[0][1], ks),
+                          torch.where(live, fresh[1][0], vn), torch.where(live, fresh[1][1], vs))
+    return pool, table
+
+
+def prepare(case, seed):
+    dev = torch.device("cuda")
+    gen = torch.Generator(device=dev).manual_seed(seed)
+
+    def normal(*shape):
+        return torch.randn(*shape, generator=gen, device=dev).bfloat16()
+
+    s = {"case": dict(case)}
+    if case["op"] == "attend":
+        b, h, t = case["batch"], case["heads"], case["tokens"]
+        lengths, valid = _prefixes(case), _targets(case)
+        s["pool"], s["table"] = _filled_pool(lengths, h, gen, dev)
+        s["q"], s["k"], s["v"] = normal(b, h, t, D), normal(b, h, t, D), normal(b, t, h, D)
+        s["desc"] = torch.tensor(list(zip(lengths, valid)), dtype=torch.int32, device=dev)
+        s["limit"] = torch.arange(1, t + 1, dtype=torch.int32, device=dev) if case["causal"] else None
+    elif case["op"] == "store":
+        starts, counts = _starts(case), _counts(case)
+        ends = [a + n for a, n in zip(starts, counts)]
+        s["pool"], s["table"] = _filled_pool(starts, case["heads"], gen, dev, ends)
+        s["k"] = normal(case["batch"], case["heads"], case["tokens"], D)
+        s["v"] = normal(case["batch"], case["tokens"], case["heads"], D).transpose(1, 2)
+        s["start"], s["count"], s["end"] = (
+            torch.tensor(z, dtype=torch.int32, device=dev) for z in (starts, counts, ends))
+        s["most"] = max(ends)
+    elif case["op"] == "pages":
+        n = case["pages"]
+        s["pool"] = torch.randint(0, 256, (case["layers"], n, case["heads"], BLOCK),
+                                  generator=gen, device=dev, dtype=torch.uint8)
+        order = torch.randperm(n, generator=gen, device=dev).tolist()
+        s["src"], s["dst"] = order[:case["moves"]], order[case["moves"]:2 * case["moves"]]
+    else:
+        k, n, r, m = case["k"], case["n"], case["rank"], case["adapters"]
+        s["x"], s["y"] = normal(case["rows"], k), normal(case["rows"], n)
+        s["a"] = (torch.randn(m, r, k, generator=gen, device=dev) * k ** -0.5).bfloat16()
+        s["b"] = (torch.randn(m, n, r, generator=gen, device=dev) * r ** -0.5).bfloat16()
+        s["scale"] = torch.rand(m, generator=gen, device=dev) + 0.5
+        ends = torch.tensor(_rows(case)).cumsum(0).tolist()
+        s["seg"] = torch.tensor([0] + ends, dtype=torch.int32, device=dev)
+        s["who"] = torch.tensor(_who(case), dtype=torch.int32, device=dev)
+        s["longest"] = max(_rows(case))
+    return s
+
+
+# --------------------------------------------------------------------------------------- run
+def _attend(s):
+    b, h, t, _ = s["q"].shape
+    kn, ks, vn, vs = _unpack(_gather(s["pool"], s["table"]))
+    pk, pv = (_rows_of(_values(n, st)) for n, st in ((kn, ks), (vn, vs)))
+    cols = torch.arange(pk.shape[2], device=pk.device)
+    seen = (cols < s["desc"][:, :1]).view(b, 1, -1, 1)
+    mine = torch.arange(t, device=pk.device)
+    live = (mine < s["desc"][:, 1:]).view(b, 1, -1, 1)
+    keys = torch.cat([torch.where(seen, pk, 0.0), torch.where(live, s["k"].float(), 0.0)], 2)
+    vals = torch.cat([torch.where(seen, pv, 0.0),
+                      torch.where(live, s["v"].transpose(1, 2).float(), 0.0)], 2)
+    ok = torch.cat([seen, live], 2).transpose(2, 3)
+    if s["limit"] is not None:
+        below = mine.view(1, -1) < s["limit"].view(-1, 1)
+        ok = ok & torch.cat([torch.ones(t, pk.shape[2], dtype=torch.bool, device=pk.device), below], 1)
+    x = (s["q"].float() @ keys.transpose(2, 3)) * D ** -0.5
+    x = x.masked_fill(~ok, -math.inf)
+    x = torch.exp(x - x.amax(-1, keepdim=True))
+    out = (x @ vals) / x.sum(-1, keepdim=True)
+    return out.transpose(1, 2).reshape(b, t, h * D).bfloat16()
+
+
+def _store(s):
+    pool, table = s["pool"], s["table"]
+    blocks = _gather(pool, table)
+    b, h, m, _ = blocks.shape
+    at = torch.arange(m * PAGE, device=pool.device).view(1, -1) - s["start"].view(-1, 1)
+    new = (at >= 0) & (at < s["count"].view(-1, 1))
+    pick = at.clamp(0, s["k"].shape[2] - 1).view(b, 1, -1, 1).expand(b, h, -1, D)
+    old = [_rows_of(z) for z in _unpack(blocks)]
+    put = [*_quantise(torch.gather(s["k"], 2, pick)), *_quantise(torch.gather(s["v"], 2, pick))]
+    now = [torch.where(new.view(b, 1, -1, 1), p, o) for p, o in zip(put, old)]
+    fresh = _pack(*(z.unflatten(2, (m, PAGE)) for z in now)).transpose(1, 2)
+    pool[table[table >= 0].long()] = fresh[table >= 0]
+    live = (torch.arange(m * PAGE, device=pool.device) < s["end"].view(-1, 1)).view(b, 1, -1, 1)
+    kn, ks, vn, vs = (_rows_of(z) for z in _unpack(_gather(pool, table)))
+    return [torch.where(live, _values(n, st), 0.0)[:, :, :s["most"]].bfloat16()
+            for n, st in ((kn, ks), (vn, vs))]
+
+
+def _lora(s):
+    rows = s["x"].shape[0]
+    first, last = s["seg"][:-1].long(), s["seg"][1:].long()
+    at = first.view(-1, 1) + torch.arange(s["longest"], device=first.device)
+    live = (at < last.view(-1, 1)) & (s["who"] >= 0).view(-1, 1)
+    who = s["who"].clamp(min=0).long()
+    x = s["x"][at.clamp(max=rows - 1)].float()
+    u = x @ s["a"].float()[who].transpose(1, 2) * s["scale"][who].view(-1, 1, 1)
+    delta = u @ s["b"].float()[who].transpose(1, 2)
+    y = s["y"].float()
+    y[at[live]] += delta[live]
+    return y.bfloat16()
+
+
+def run(s):
+    op = s["case"]["op"]
+    if own:
+        api = _api()
+        if op == "attend":
+            return api.kv4_joint_attention(s["q"], s["k"], s["v"], s["pool"], s["table"],
+                                           s["case"]["prefix"], desc=s["desc"], row_limit=s["limit"])
+        if op == "store":
+            api.kv4_store(s["k"], s["v"], s["pool"], s["table"], start=s["start"], count=s["count"])
+            return list(api.kv4_load(s["pool"], s["table"], s["end"], s["most"]))
+        if op == "pages":
+            api.kv4_copy_pages(s["pool"], s["src"], s["dst"])
+            return s["pool"]
+        return api.lora_add(s["x"], s["a"], s["b"], s["y"], s["seg"], s["who"], scale=s["scale"],
+                            out=torch.empty_like(s["y"]))
+    if op == "attend":
+        return _attend(s)
+    if op == "store":
+        return _store(s)
+    if op == "pages":
+        s["pool"][:, s["dst"]] = s["pool"][:, s["src"]]
+        return s["pool"]
+    return _lora(s)
+
+
+# ------------------------------------------------------------------------------------- exact
+def _exact_rows(pool, ids, count, h, part):
+    """Tokens [0, count) of head h of the pages `ids`, K (part 0) or V (part 1), in 64 bits:
+    each value found by its own byte and bit."""
+    dev = pool.device
+    tok = torch.arange(count, device=dev).view(-1, 1)
+    ch = torch.arange(D, device=dev).view(1, -1)
+    r = tok % PAGE
+    octet, group = r // 8, ch // 32
+    if part == 0:
+        lane = (r % 8) * 4 + (ch % 32) // 8
+        byte = octet * 512 + lane * 16 + group * 4 + (ch % 8) // 2
+        high = ch % 2
+    else:
+        lane = ((ch % 32) // 4) * 4 + (r % 8) // 2
+        byte = 4096 + octet * 512 + lane * 16 + group * 4 + (r % 2) * 2 + (ch % 4) // 2
+        high = ch % 2
+    page = ids.long()[tok // PAGE]
+    raw = pool[page, h, byte].to(torch.int64)
+    num = torch.where(high == 1, raw // 16, raw % 16) - 8
+    at = 8192 + part * 512 + octet * 64 + ((r % 8) // 2) * 16 + group * 4 + (r % 2) * 2
+    bits = pool[page, h, at].to(torch.int64) + 256 * pool[page, h, at + 1].to(torch.int64)
+    step = (bits.to(torch.int32) << 16).view(torch.float32).double()
+    return num.double() * step
+
+
+def _exact_quantised(x):
+    """x [..., 128] -> the values that the cache holds for it, in 64 bits."""
+    g = x.double().reshape(*x.shape[:-1], 4, 32)
+    top = g.abs().amax(-1, keepdim=True)
+    frac, power = torch.frexp(top / 7.0)            # frac in [1/2, 1)
+    whole = torch.round(frac * 32.0)                # 5 significant bits; halves to even
+    step = torch.ldexp(whole / 32.0, power)
+    num = torch.sign(g) * torch.floor(g.abs() / step + 0.5)
+    return torch.where(top < TINY, 0.0, num * step).reshape(x.shape)
+
+
+def exact(case, seed):
+    s = prepare(case, seed)
+    op = case["op"]
+    if op == "pages":
+        return None  # bytes: no computed number
+    if op == "attend":
+        b, h, t = case["batch"], case["heads"], case["tokens"]
+        out = torch.empty(b, t, h, D, dtype=torch.float64, device="cuda")
+        for i in range(b):
+            n, m = s["desc"][i].tolist()
+            for j in range(h):
+                pk, pv = (_exact_rows(s["pool"], s["table"][i], n, j, p) for p in (0, 1))
+                for r in range(0, t, 1024):
+                    q = s["q"][i, j, r:r + 1024].double()
+                    x = torch.cat([q @ pk.T, q @ s["k"][i, j, :m].double().T], 1) / math.sqrt(D)
+                    if s["limit"] is not None:
+                        hide = torch.arange(m, device="cuda").view(1, -1) >= s["limit"][r:r + 1024].view(-1, 1)
+                        x[:, n:][hide] = -math.inf
+                    p = torch.softmax(x, -1)
+                    out[i, r:r + 1024, j] = p[:, :n] @ pv + p[:, n:] @ s["v"][i, :m, j].double()
+        return out.reshape(b, t, h * D)
+    if op == "store":
+        b, h = case["batch"], case["heads"]
+        got = [torch.zeros(b, h, s["most"], D, dtype=torch.float64, device="cuda") for _ in range(2)]
+        for i in range(b):
+            a, n = int(s["start"][i]), int(s["count"][i])
+            for part, name in ((0, "k"), (1, "v")):
+                for j in range(h):
+                    got[part][i, j, :a] = _exact_rows(s["pool"], s["table"][i], a, j, part)
+                got[part][i, :, a:a + n] = _exact_quantised(s[name][i, :, :n])
+        return got
+    y = s["y"].double()
+    seg = s["seg"].tolist()
+    for i, who in enumerate(s["who"].tolist()):
+        if who >= 0:
+            x = s["x"][seg[i]:seg[i + 1]].double()
+            y[seg[i]:seg[i + 1]] += float(s["scale"][who]) * ((x @ s["a"][who].double().T) @ s["b"][who].double().T)
+    return y
