@@ -197,13 +197,13 @@ def _counts(case):
 # --------------------------------------------------------------- the cache's bytes, plain form
 def _quantise(x):
     """x [..., 128] -> numbers uint8 [..., 128] (1..15) and steps f32 [..., 4].  The step is
-    the group's largest magnitude / 7 rounded to 5 significant bits, so that every product
+    the group's largest magnitude / 7 cut to 5 significant bits, so that every product
     step * (number - 8) is a bf16 value; halves round away from zero."""
     g = x.float().unflatten(-1, (4, 32))
     top = g.abs().amax(-1)
     seven = torch.full_like(top, 7.0)  # a tensor: a true division, rounded once
     bits = (top / seven).view(torch.int32)
-    step = (((bits + 0x3FFFF + ((bits >> 19) & 1)) >> 19) << 19).view(torch.float32)
+    step = ((bits >> 19) << 19).view(torch.float32)
     step = torch.where(top < TINY, torch.zeros_like(step), step)
     step = torch.where(torch.isfinite(top), step, torch.full_like(step, math.nan))
     use = (step > 0).unsqueeze(-1)
@@ -457,7 +457,7 @@ def _exact_quantised(x):
     g = x.double().reshape(*x.shape[:-1], 4, 32)
     top = g.abs().amax(-1, keepdim=True)
     frac, power = torch.frexp(top / 7.0)            # frac in [1/2, 1)
-    whole = torch.round(frac * 32.0)                # 5 significant bits; halves to even
+    whole = torch.floor(frac * 32.0)                # 5 significant bits
     step = torch.ldexp(whole / 32.0, power)
     num = torch.sign(g) * torch.floor(g.abs() / step + 0.5)
     return torch.where(top < TINY, 0.0, num * step).reshape(x.shape)
