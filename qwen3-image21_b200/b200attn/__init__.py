@@ -42,6 +42,9 @@ EXPORTED = (
     "b200_qkv_norm_rope_gemm",
     "b200_tp_unique_id", "b200_tp_init", "b200_tp_init_from_nccl", "b200_tp_rank", "b200_tp_size",
     "b200_tp_out_proj_allreduce", "b200_tp_wait", "b200_tp_destroy",
+    "b200_kv4_store", "b200_kv4_load", "b200_kv4_attention_workspace_bytes",
+    "b200_kv4_joint_attention", "b200_kv4_attn_workspace_bytes", "b200_kv4_attn_fwd",
+    "b200_kv4_copy_pages",
 )
 
 
@@ -70,6 +73,12 @@ class AttnArgs(ctypes.Structure):
         ("workspace_bytes", ctypes.c_size_t), ("status", ctypes.c_void_p),
         ("row_limit", ctypes.c_void_p), ("pe_batch_stride", ctypes.c_int64),
     ]
+
+
+class Kv4View(ctypes.Structure):
+    """b200_kv4_view: one layer's pool of 4-bit pages and a batch's page tables."""
+    _fields_ = [("pool", ctypes.c_void_p), ("page_table", ctypes.c_void_p),
+                ("num_pages", ctypes.c_int32), ("max_pages", ctypes.c_int32)]
 
 
 _lib = None
@@ -112,6 +121,18 @@ def lib() -> ctypes.CDLL:
         L.b200_reduce_nvls.argtypes = [vp, i64, vp, i64, i64, i32, i32, vp, i64, vp, vp, i64, i64,
                                        f32, vp]
         L.b200_kquant_gemv.argtypes = [vp, i64, vp, i32, vp, i64, i32, i32, i32, vp]
+        vw = ctypes.POINTER(Kv4View)
+        L.b200_kv4_store.argtypes = [vw, vp, i64, i64, i64, vp, i64, i64, i64, i32, i32, i32, i32, vp,
+                                     vp, vp, vp]
+        L.b200_kv4_load.argtypes = [vw, vp, i32, vp, vp, i32, i32, i32, i32, vp, vp]
+        L.b200_kv4_attention_workspace_bytes.argtypes = [i32, i32, i32, i32,
+                                                         ctypes.POINTER(ctypes.c_size_t)]
+        L.b200_kv4_joint_attention.argtypes = [vw, vp, vp, vp, i32, i32, i32, i32, i32, vp, vp, f32,
+                                               vp, vp, ctypes.c_size_t, vp, vp]
+        L.b200_kv4_attn_workspace_bytes.argtypes = [ctypes.POINTER(AttnArgs),
+                                                    ctypes.POINTER(ctypes.c_size_t)]
+        L.b200_kv4_attn_fwd.argtypes = [ctypes.POINTER(AttnArgs), vw, vp]
+        L.b200_kv4_copy_pages.argtypes = [vp, i32, i64, i32, i32, vp, vp, i32, vp]
         L.b200_tp_unique_id.argtypes = [vp]
         L.b200_tp_init.argtypes = [ctypes.POINTER(vp), vp, i32, i32, ctypes.c_uint32]
         L.b200_tp_init_from_nccl.argtypes = [ctypes.POINTER(vp), vp, ctypes.c_uint32]
@@ -546,6 +567,210 @@ def qkv_norm_rope_gemm(x, w_qkv, batch: int, tokens: int, heads: int, norm_q_w, 
                                          _dptr(pe), pe_bs, _dptr(q_rot), _dptr(k_rot), _dptr(v),
                                          _dptr(status), _stream(stream)), "b200_qkv_norm_rope_gemm")
     return q_rot, k_rot, v
+
+
+# ----------------------------------------------------------------- paged 4-bit prefix cache
+KV4_PAGE_TOKENS, KV4_BLOCK_BYTES = 64, 9216
+KV4_DENSE_QUERIES = 65   # B200_KV4_DENSE_QUERIES
+KV4_STATUS_BAD_PAGE = 16
+
+
+def _expect(t, name: str, dtype, shape, device, dense: bool = True) -> None:
+    """ValueError unless t is a tensor of this dtype, shape and device (and contiguous)."""
+    if t.dtype is dtype and t.shape == shape and t.device == device and (not dense or t.is_contiguous()):
+        return
+    if t.dtype is not dtype:
+        raise ValueError(f"{name} must be {dtype}, not {t.dtype}")
+    if t.shape != shape:
+        raise ValueError(f"{name} must have the shape {tuple(shape)}, not {tuple(t.shape)}")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, not on {device}")
+    raise ValueError(f"{name} must be contiguous")
+
+
+class _Launch:
+    """Makes t's device current and, where a stream is given, that stream: the library
+    launches on the current device, and what is allocated meanwhile belongs to the stream
+    that the kernels run on."""
+
+    def __init__(self, t, stream):
+        import torch
+        if not t.is_cuda:
+            raise ValueError("the library computes on CUDA tensors only")
+        self.within = []
+        if t.device.index != torch.cuda.current_device():
+            self.within.append(torch.cuda.device(t.device))
+        if stream is not None:
+            if not isinstance(stream, torch.cuda.Stream):
+                raw = _stream(stream)
+                stream = (torch.cuda.ExternalStream(raw, device=t.device) if raw
+                          else torch.cuda.default_stream(t.device))
+            if stream.device != t.device:
+                raise ValueError(f"the stream is on {stream.device}, the tensors on {t.device}")
+            self.within.append(torch.cuda.stream(stream))
+
+    def __enter__(self):
+        for c in self.within:
+            c.__enter__()
+        return _stream(None)
+
+    def __exit__(self, *exc):
+        for c in reversed(self.within):
+            c.__exit__(*exc)
+
+
+def _kv4_view(pool, page_table, batch: int, heads: int) -> Kv4View:
+    """Checked b200_kv4_view of pool uint8 [num_pages, heads, 9216], page_table int32
+    [batch, max_pages]."""
+    import torch
+    _expect(pool, "pool", torch.uint8, (pool.shape[0], heads, KV4_BLOCK_BYTES), pool.device)
+    _expect(page_table, "page_table", torch.int32, (batch, page_table.shape[-1]), pool.device)
+    return Kv4View(pool.data_ptr(), page_table.data_ptr(), pool.shape[0], page_table.shape[1])
+
+
+def kv4_store(k, v, pool, page_table, start=None, count=None, status=None, stream=None):
+    """Stores k, v (bf16 [B, H, T, 128], any strides with the 128 channels dense, e.g. a
+    transposed token-major tensor) into the 4-bit pages: token i < count[b] of batch row b at
+    position start[b] + i of its sequence.  pool uint8 [num_pages, H, 9216]; page_table int32
+    [B, max_pages]; start, count int32 [B] or None (0 and T)."""
+    import torch
+    b, h, t, d = k.shape
+    _expect(k, "k", torch.bfloat16, (b, h, t, d), pool.device, dense=False)
+    _expect(v, "v", torch.bfloat16, (b, h, t, d), pool.device, dense=False)
+    if k.numel() and (k.stride(3) != 1 or v.stride(3) != 1):
+        raise ValueError("the channels of k and v must be dense")
+    view = _kv4_view(pool, page_table, b, h)
+    for x, name in ((start, "start"), (count, "count")):
+        if x is not None:
+            _expect(x, name, torch.int32, (b,), pool.device)
+    # a stride is not looked at where its extent is 1 (torch leaves any number there)
+    ks, vs = ([s if n > 1 else 0 for s, n in zip(x.stride()[:3], x.shape)] for x in (k, v))
+    with _Launch(pool, stream) as st:
+        _check(lib().b200_kv4_store(ctypes.byref(view), _dptr(k), *ks, _dptr(v), *vs, b, h, t, d,
+                                    _dptr(start), _dptr(count), _dptr(status), st),
+               "b200_kv4_store")
+
+
+def kv4_load(pool, page_table, lengths, max_len: int, k_out=None, v_out=None, status=None,
+             stream=None):
+    """Reads the cache back: (k, v) bf16 [B, H, max_len, 128], the dense prefix layout; rows
+    from lengths[b] (int32 [B], or None: max_len) on are zeros."""
+    import torch
+    h, b = pool.shape[1], page_table.shape[0]
+    view = _kv4_view(pool, page_table, b, h)
+    shape = (b, h, int(max_len), HEAD_DIM)
+    if lengths is not None:
+        _expect(lengths, "lengths", torch.int32, (b,), pool.device)
+    with _Launch(pool, stream) as st:
+        k_out, v_out = (torch.empty(shape, dtype=torch.bfloat16, device=pool.device) if x is None
+                        else x for x in (k_out, v_out))
+        _expect(k_out, "k_out", torch.bfloat16, shape, pool.device)
+        _expect(v_out, "v_out", torch.bfloat16, shape, pool.device)
+        _check(lib().b200_kv4_load(ctypes.byref(view), _dptr(lengths), 1, _dptr(k_out),
+                                   _dptr(v_out), b, h, int(max_len), HEAD_DIM, _dptr(status), st),
+               "b200_kv4_load")
+    return k_out, v_out
+
+
+def kv4_joint_attention(q_rot, k_rot, v, pool, page_table, prefix_len: int, desc=None,
+                        row_limit=None, scale=None, out=None, workspace=None, status=None,
+                        stream=None):
+    """joint_attention with the prefix in the paged 4-bit cache: q_rot, k_rot bf16 [B,H,T,D],
+    v bf16 [B,T,H,D], pool uint8 [num_pages, H, 9216], page_table int32 [B, max_pages] -> out
+    bf16 [B,T,H*D].  prefix_len bounds every desc[b].prefix_valid (desc int32 [B, 2] or None:
+    prefix_len and T).  row_limit int32 [T] or None: row i sees this call's keys
+    [0, row_limit[i]).  workspace uint8 (kv4_workspace_bytes; needed from
+    KV4_DENSE_QUERIES tokens on, allocated here when None)."""
+    import torch
+    b, h, t, d = q_rot.shape
+    dev = pool.device
+    bf = torch.bfloat16
+    _expect(q_rot, "q_rot", bf, (b, h, t, d), dev)
+    _expect(k_rot, "k_rot", bf, (b, h, t, d), dev)
+    _expect(v, "v", bf, (b, t, h, d), dev)
+    view = _kv4_view(pool, page_table, b, h)
+    if desc is not None:
+        _expect(desc, "desc", torch.int32, (b, 2), dev)
+    if row_limit is not None:
+        _expect(row_limit, "row_limit", torch.int32, (t,), dev)
+    with _Launch(pool, stream) as st:
+        if out is None:
+            out = torch.empty((b, t, h * d), dtype=bf, device=dev)
+        _expect(out, "out", bf, (b, t, h * d), dev)
+        if workspace is None and t >= KV4_DENSE_QUERIES:
+            workspace = torch.empty(kv4_workspace_bytes(b, h, t, prefix_len), dtype=torch.uint8,
+                                    device=dev)
+        ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
+        _check(lib().b200_kv4_joint_attention(
+            ctypes.byref(view), _dptr(q_rot), _dptr(k_rot), _dptr(v), b, h, t, int(prefix_len), d,
+            _dptr(desc), _dptr(row_limit), float(d ** -0.5 if scale is None else scale), _dptr(out),
+            _dptr(workspace), ws_bytes, _dptr(status), st), "b200_kv4_joint_attention")
+    return out
+
+
+def kv4_workspace_bytes(batch: int, heads: int, target_len: int, prefix_len: int) -> int:
+    """Scratch bytes of kv4_joint_attention for these sizes."""
+    n = ctypes.c_size_t()
+    _check(lib().b200_kv4_attention_workspace_bytes(batch, heads, target_len, int(prefix_len),
+                                                    ctypes.byref(n)),
+           "b200_kv4_attention_workspace_bytes")
+    return n.value
+
+
+def kv4_attention_forward(q, k, v, pool, page_table, prefix_len: int, norm_q_w, norm_k_w, pe,
+                          desc=None, scale=None, eps: float = 1e-6, out=None, k_rot_out=None,
+                          v_out=None, workspace=None, status=None, stream=None, row_limit=None):
+    """attention_forward with the prefix in the paged 4-bit cache (see kv4_joint_attention):
+    q, k, v bf16 [B,T,H,D] raw projections, Q/K RMSNorm + RoPE, then joint attention."""
+    import torch
+    b, t, h, d = q.shape
+    for x, name in ((q, "q"), (k, "k"), (v, "v")):
+        _expect(x, name, torch.bfloat16, (b, t, h, d), pool.device)
+    for x, name in ((k_rot_out, "k_rot_out"), (v_out, "v_out")):
+        if x is not None:
+            _expect(x, name, torch.bfloat16, (b, h, t, d), pool.device)
+    _expect(norm_q_w, "norm_q_w", torch.float32, (d,), pool.device)
+    _expect(norm_k_w, "norm_k_w", torch.float32, (d,), pool.device)
+    _expect(pe, "pe", torch.float32, (b, t, d) if pe.dim() == 3 else (t, d), pool.device)
+    view = _kv4_view(pool, page_table, b, h)
+    if desc is not None:
+        _expect(desc, "desc", torch.int32, (b, 2), pool.device)
+    if row_limit is not None:
+        _expect(row_limit, "row_limit", torch.int32, (t,), pool.device)
+    with _Launch(pool, stream) as st:
+        if out is None:
+            out = torch.empty((b, t, h * d), dtype=torch.bfloat16, device=q.device)
+        _expect(out, "out", torch.bfloat16, (b, t, h * d), pool.device)
+        args = make_args(q, k, v, None, None, norm_q_w, norm_k_w, pe, out, desc, scale, eps,
+                         k_rot_out, v_out, None, status, row_limit)
+        args.prefix_len = int(prefix_len)
+        if workspace is None:
+            n = ctypes.c_size_t()
+            _check(lib().b200_kv4_attn_workspace_bytes(ctypes.byref(args), ctypes.byref(n)),
+                   "b200_kv4_attn_workspace_bytes")
+            workspace = torch.empty(max(n.value, 1), dtype=torch.uint8, device=q.device)
+        args.workspace = workspace.data_ptr()
+        args.workspace_bytes = workspace.numel() * workspace.element_size()
+        _check(lib().b200_kv4_attn_fwd(ctypes.byref(args), ctypes.byref(view), st),
+               "b200_kv4_attn_fwd")
+    return out
+
+
+def kv4_copy_pages(pool, src: Sequence[int], dst: Sequence[int], stream=None):
+    """Copies page src[i] onto page dst[i] in every layer of pool uint8 [layers, num_pages, H,
+    9216] (or one layer's [num_pages, H, 9216]).  src and dst are host sequences; a page that
+    is written twice, or both read and written, is refused (B200Error ERR_INVALID)."""
+    import torch
+    if pool.dim() == 3:
+        pool = pool.unsqueeze(0)
+    _expect(pool, "pool", torch.uint8, (*pool.shape[:3], KV4_BLOCK_BYTES), pool.device)
+    if len(src) != len(dst):
+        raise ValueError("src and dst must have the same length")
+    n = len(src)
+    s, d = (ctypes.c_int32 * n)(*src), (ctypes.c_int32 * n)(*dst)
+    with _Launch(pool, stream) as st:
+        _check(lib().b200_kv4_copy_pages(_dptr(pool), pool.shape[0], pool.stride(0), pool.shape[1],
+                                         pool.shape[2], s, d, n, st), "b200_kv4_copy_pages")
 
 
 # ----------------------------------------------------------------- head-sharding communicator

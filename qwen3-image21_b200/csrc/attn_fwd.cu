@@ -31,6 +31,7 @@
 #include <mutex>
 
 #include "../../include/b200_attn.h"
+#include "attn_internal.h"
 #include "ptx.cuh"
 
 namespace b200 {
@@ -249,6 +250,19 @@ __device__ __forceinline__ float row_sum(const uint32_t (&r)[4][32]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) f2unpack(acc[i], s[2 * i], s[2 * i + 1]);
   return ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
+}
+
+// Clears rows [first, 128) of a V tile in shared memory (one warp): keys behind the valid
+// ones have P = 0, but 0 * V is NaN where V holds an infinity or a NaN there.  A row is 128
+// bytes of each of the tile's two regions, whatever the swizzle.  At most one tile of each
+// segment has such rows.
+__device__ __noinline__ void clear_v_rows(uint8_t* tile, int first, int lane) {
+  for (int i = first * 8 + lane; i < kBN * 8; i += 32) {
+    *reinterpret_cast<uint4*>(tile + i * 16) = make_uint4(0, 0, 0, 0);
+    *reinterpret_cast<uint4*>(tile + kRegionBytes + i * 16) = make_uint4(0, 0, 0, 0);
+  }
+  fence_proxy_async();
+  __syncwarp();
 }
 
 // kF16: Q, K, V, P and the output are IEEE half (the reference's FA2 branch casts to
@@ -503,7 +517,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int s1 = (j + 1) & 1;
         const uint32_t u1 = static_cast<uint32_t>((j + 1) >> 1);
         const bool more = j + 1 < n;
-        if (!wait(v_full + s, u & 1) || !wait(p_full + 0, j & 1)) {
+        if (!wait(v_full + s, u & 1)) {
+          ok = false;
+          break;
+        }
+        {
+          const int ja = jb + j;
+          const int valid = ja < n0 ? pv - ja * kBN : tv - (ja - n0) * kBN;
+          if (valid < kBN) clear_v_rows(sV + s * kTileBytes, max(valid, 0), lane);
+        }
+        if (!wait(p_full + 0, j & 1)) {
           ok = false;
           break;
         }
@@ -1109,13 +1132,14 @@ int launch_norm_rope(const NormRopeJob* jobs, int njobs, int B, int T, int H, fl
   return cudaGetLastError() == cudaSuccess ? B200_OK : B200_ERR_CUDA;
 }
 
+}  // namespace
+
 // Attention of post-RoPE q [B,H,T,D] over [prefix (B,H,P,D) ; step k_rot (B,H,T,D) and
 // v (B,T,H,D, token-major)], out [B,T,H*D].  Arguments are already validated.
 int joint_attention(const void* q_rot, const void* k_rot, const void* v, const void* prefix_k,
                     const void* prefix_v, int B, int H, int T, int P, const b200_kv_desc* desc,
                     float scale, void* out, int32_t* status, void* split_region,
-                    cudaStream_t stream, bool counters_zeroed = false,
-                    const int32_t* row_limit = nullptr) {
+                    cudaStream_t stream, bool counters_zeroed, const int32_t* row_limit) {
   CUtensorMap mq{}, mk0{}, mv0{}, mk1{}, mv1{}, mo{};
   int rc;
   if ((rc = make_map(&mq, q_rot, B, H, T, true)) != B200_OK) return rc;
@@ -1148,7 +1172,15 @@ int joint_attention(const void* q_rot, const void* k_rot, const void* v, const v
                           counters_zeroed);
 }
 
-}  // namespace
+int attn_prologue(const b200_attn_args& a, void* q_rot, void* k_rot, cudaStream_t stream) {
+  NormRopeJob jobs[3] = {
+      {static_cast<const __nv_bfloat16*>(a.q), static_cast<__nv_bfloat16*>(q_rot), a.norm_q_w},
+      {static_cast<const __nv_bfloat16*>(a.k), static_cast<__nv_bfloat16*>(k_rot), a.norm_k_w},
+      {static_cast<const __nv_bfloat16*>(a.v), static_cast<__nv_bfloat16*>(a.v_out), nullptr}};
+  return launch_norm_rope(jobs, a.v_out ? 3 : 2, a.batch, a.target_len, a.heads, a.norm_eps, a.pe,
+                          a.pe_batch_stride, 0x3, stream);
+}
+
 }  // namespace b200
 
 using namespace b200;
