@@ -44,7 +44,7 @@ EXPORTED = (
     "b200_tp_out_proj_allreduce", "b200_tp_wait", "b200_tp_destroy",
     "b200_kv4_store", "b200_kv4_load", "b200_kv4_attention_workspace_bytes",
     "b200_kv4_joint_attention", "b200_kv4_attn_workspace_bytes", "b200_kv4_attn_fwd",
-    "b200_kv4_copy_pages",
+    "b200_kv4_copy_pages", "b200_lora_add",
 )
 
 
@@ -133,6 +133,8 @@ def lib() -> ctypes.CDLL:
                                                     ctypes.POINTER(ctypes.c_size_t)]
         L.b200_kv4_attn_fwd.argtypes = [ctypes.POINTER(AttnArgs), vw, vp]
         L.b200_kv4_copy_pages.argtypes = [vp, i32, i64, i32, i32, vp, vp, i32, vp]
+        L.b200_lora_add.argtypes = [vp, i64, vp, vp, vp, i64, vp, i64, vp, vp, vp, i32, i32, i32, i32,
+                                    i32, i32, vp, vp]
         L.b200_tp_unique_id.argtypes = [vp]
         L.b200_tp_init.argtypes = [ctypes.POINTER(vp), vp, i32, i32, ctypes.c_uint32]
         L.b200_tp_init_from_nccl.argtypes = [ctypes.POINTER(vp), vp, ctypes.c_uint32]
@@ -771,6 +773,46 @@ def kv4_copy_pages(pool, src: Sequence[int], dst: Sequence[int], stream=None):
     with _Launch(pool, stream) as st:
         _check(lib().b200_kv4_copy_pages(_dptr(pool), pool.shape[0], pool.stride(0), pool.shape[1],
                                          pool.shape[2], s, d, n, st), "b200_kv4_copy_pages")
+
+
+# ----------------------------------------------------------------- per-request adapters
+LORA_MAX_RANK = 128
+LORA_STATUS_BAD_ADAPTER = 16
+
+
+def lora_add(x, a, b, y, seg_start, seg_adapter, scale=None, out=None, status=None, stream=None):
+    """Adds each request's low-rank part beside a shared projection: out[r] = y[r] + scale[e] *
+    (x[r] @ a[e].T) @ b[e].T for the rows [seg_start[s], seg_start[s + 1]) of request s with
+    adapter e = seg_adapter[s] (negative: none).  x bf16 [R, K], y and out bf16 [R, N] (any
+    row strides; out None: in place), a bf16 [E, rank, K], b bf16 [E, N, rank], seg_start
+    int32 [S + 1], seg_adapter int32 [S], scale f32 [E] or None (1).  Returns out."""
+    import torch
+    bf, dev = torch.bfloat16, x.device
+    (rows, k), n, (e, rank) = x.shape, y.shape[1], a.shape[:2]
+    _expect(x, "x", bf, (rows, k), dev, dense=False)
+    _expect(y, "y", bf, (rows, n), dev, dense=False)
+    _expect(a, "a", bf, (e, rank, k), dev)
+    _expect(b, "b", bf, (e, n, rank), dev)
+    segments = seg_adapter.shape[0]
+    _expect(seg_start, "seg_start", torch.int32, (segments + 1,), dev)
+    _expect(seg_adapter, "seg_adapter", torch.int32, (segments,), dev)
+    if scale is not None:
+        _expect(scale, "scale", torch.float32, (e,), dev)
+    if out is None:
+        out = y
+    else:
+        _expect(out, "out", bf, (rows, n), dev, dense=False)
+    strides = []
+    for t, name, cols in ((x, "x", k), (y, "y", n), (out, "out", n)):
+        if cols > 1 and t.stride(1) != 1:
+            raise ValueError(f"the rows of {name} must be dense")
+        strides.append(t.stride(0) if rows > 1 else (cols + 7) // 8 * 8)
+    with _Launch(x, stream) as st:
+        _check(lib().b200_lora_add(_dptr(x), strides[0], _dptr(a), _dptr(b), _dptr(y), strides[1],
+                                   _dptr(out), strides[2], _dptr(seg_start), _dptr(seg_adapter),
+                                   _dptr(scale), rows, segments, e, n, k, rank, _dptr(status), st),
+               "b200_lora_add")
+    return out
 
 
 # ----------------------------------------------------------------- head-sharding communicator

@@ -15,12 +15,13 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "b200attn", "libb200attn.so")
-SOURCES = ["attn_fwd.cu", "block_ops.cu", "dequant.cu", "gemm.cu", "kv4.cu", "host_layout.cpp", "tp.cpp"]
+SOURCES = ["attn_fwd.cu", "block_ops.cu", "dequant.cu", "gemm.cu", "kv4.cu", "lora.cu", "host_layout.cpp", "tp.cpp"]
 HEADERS = ["ptx.cuh", "attn_internal.h", os.path.join("..", "..", "include", "b200_attn.h"),
            os.path.join("..", "..", "include", "b200_block_ops.h"),
            os.path.join("..", "..", "include", "b200_gguf.h"),
            os.path.join("..", "..", "include", "b200_gemm.h"),
            os.path.join("..", "..", "include", "b200_kv4.h"),
+           os.path.join("..", "..", "include", "b200_lora.h"),
            os.path.join("..", "..", "include", "b200_tp.h")]
 
 

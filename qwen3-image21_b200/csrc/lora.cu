@@ -1,0 +1,616 @@
+// lora.cu — per-request low-rank adapters beside a shared projection (include/b200_lora.h):
+//   out = y + scale * (x A^T) B^T
+// in one launch.  At ranks of 8 to 128 the operator is bound by HBM: x, y and out are read
+// or written once (the adapters are small), so the inner product u = x A^T must not leave
+// the chip.
+//
+// One cluster of C CTAs per 128-row tile of a request.
+//   1. CTA c multiplies its part of K: x tiles [128 x 64] and A tiles [rank x 64] arrive by
+//      TMA, u_c accumulates in TMEM (tcgen05.mma M128 N=rank).
+//   2. The partial sums meet through distributed shared memory: CTA c adds the C partials of
+//      its 128 / C rows in rank order, scales, rounds to bf16, and fetches the other rows.
+//   3. CTA c walks its part of N in 64-column steps: B tiles and y tiles by TMA, u B^T in
+//      TMEM (two accumulators), the epilogue adds y in shared memory and writes whole
+//      128-byte row segments.  Rows of another request in the tile are not written.
+// C grows as the tiles get fewer, so that small calls still use the whole GPU; the loads of
+// step 3 start while step 2 runs.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <cudaTypedefs.h>
+
+#include <algorithm>
+#include <cstdint>
+#include <mutex>
+
+#include "../../include/b200_lora.h"
+#include "ptx.cuh"
+
+namespace b200 {
+namespace {
+
+constexpr int kTM = 128;                 // rows of a tile
+constexpr int kTK = 64;                  // K per step (one 128-byte swizzle span)
+constexpr int kTN = 64;                  // output columns per step
+constexpr int kXBytes = kTM * kTK * 2;   // x tile, or y tile: 16 KiB
+constexpr int kLThreads = 256;
+constexpr uint32_t kLTmemCols = 256;     // u: 128 columns, two accumulators of 64
+constexpr uint32_t kAccCol = 128;
+constexpr int kMaxStages = 4;
+
+struct LoraParams {
+  const __nv_bfloat16* y;
+  __nv_bfloat16* out;
+  int64_t ldy, ldo;
+  const int32_t* seg_start;
+  const int32_t* seg_adapter;
+  const float* scale;
+  int32_t rows, segments, adapters, n, k, rank;
+  int32_t rp;            // rank rounded up to 16
+  int32_t stages, stage_bytes;
+  int32_t C;             // CTAs of a cluster
+  int32_t* status;
+};
+
+__device__ __forceinline__ uint32_t lora_rank_in_cluster() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+
+__device__ __forceinline__ void lora_cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ uint32_t peer_addr(const void* p, uint32_t cta) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_addr(p)), "r"(cta));
+  return r;
+}
+
+__device__ __forceinline__ float4 peer_ld_f32x4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+
+__device__ __forceinline__ uint4 peer_ld_16b(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+
+// Arrive on the barrier at this offset in CTA `cta`, releasing at cluster scope.
+__device__ __forceinline__ void peer_arrive(uint64_t* bar, uint32_t cta) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(peer_addr(bar, cta))
+               : "memory");
+}
+
+__device__ __forceinline__ bool try_wait_cluster(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_addr(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
+// mbar_wait for barriers that other CTAs of the cluster arrive on.
+__device__ __forceinline__ bool wait_cluster(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  const uint64_t t0 = global_timer_ns();
+  for (uint32_t i = 1; !try_wait_cluster(bar, parity); ++i)
+    if ((i & 255u) == 0 && (*abort_flag || global_timer_ns() - t0 > kWaitLimitNs)) return false;
+  return true;
+}
+
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar, int32_t c0,
+                                            int32_t c1, int32_t c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_addr(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_addr(bar)), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
+
+__device__ __forceinline__ uint32_t lora_pack(float lo, float hi) {
+  __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&v);
+}
+
+__device__ __forceinline__ void epi_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+
+// The request and rows of tile `tile`; all lanes of one warp call it.  Returns the number of
+// rows, 0 when there is no such tile.
+__device__ __forceinline__ int find_tile(const LoraParams& p, int tile, int lane, int& seg, int& row0) {
+  int before = 0;
+  for (int s0 = 0; s0 < p.segments; s0 += 32) {
+    const int s = s0 + lane;
+    int lo = 0, len = 0;
+    if (s < p.segments) {
+      lo = min(max(p.seg_start[s], 0), p.rows);
+      len = max(min(p.seg_start[s + 1], p.rows) - lo, 0);
+    }
+    const int mine = (len + kTM - 1) / kTM;
+    int sum = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += x;
+    }
+    const int all = __shfl_sync(0xffffffffu, sum, 31);
+    if (tile < before + all) {
+      const unsigned hit = __ballot_sync(0xffffffffu, tile < before + sum);
+      const int who = __ffs(hit) - 1;
+      const int skip = tile - before - (__shfl_sync(0xffffffffu, sum - mine, who));
+      const int base = __shfl_sync(0xffffffffu, lo, who), rows = __shfl_sync(0xffffffffu, len, who);
+      seg = s0 + who;
+      row0 = base + skip * kTM;
+      return min(kTM, rows - skip * kTM);
+    }
+    before += all;
+  }
+  return 0;
+}
+
+__global__ void __launch_bounds__(kLThreads)
+    lora_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_a,
+                const __grid_constant__ CUtensorMap tm_b, const __grid_constant__ CUtensorMap tm_y,
+                const LoraParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* ring = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* u_buf = ring + p.stages * p.stage_bytes;  // bf16 u, K-major, 128-byte swizzle
+  const int u_regions = p.rp > 64 ? 2 : 1;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(u_buf + u_regions * kXBytes);
+  uint64_t* full = bars;                      // [kMaxStages]
+  uint64_t* empty = bars + kMaxStages;        // [kMaxStages] step 1: the MMAs are done
+  uint64_t* empty2 = bars + 2 * kMaxStages;   // [kMaxStages] step 3: the epilogue is done
+  uint64_t* u_full = bars + 3 * kMaxStages;   // partial u in TMEM
+  uint64_t* u_ready = u_full + 1;             // bf16 u in u_buf
+  uint64_t* acc_full = u_full + 2;            // [2]
+  uint64_t* acc_empty = u_full + 4;           // [2]
+  uint64_t* part_ready = u_full + 6;          // every CTA's partials are written
+  uint64_t* slice_ready = u_full + 7;         // every CTA's rows are reduced (and partials read)
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(u_full + 8);
+  int* tile_word = reinterpret_cast<int*>(u_full + 9);  // [3]: rows, segment, first row
+  volatile int* abort_flag = tile_word + 3;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int C = p.C;
+  const int rank = C > 1 ? static_cast<int>(lora_rank_in_cluster()) : 0;
+  const int NS = p.stages;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < NS; ++s) {
+      mbar_init(full + s, 1);
+      mbar_init(empty + s, 1);
+      mbar_init(empty2 + s, 4);
+    }
+    mbar_init(u_full, 1);
+    mbar_init(u_ready, 128);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(acc_full + i, 1);
+      mbar_init(acc_empty + i, 4);
+    }
+    mbar_init(part_ready, C);
+    mbar_init(slice_ready, C);
+    *abort_flag = 0;
+    fence_barrier_init();
+    fence_proxy_async();
+  }
+  if (warp == 2) {
+    tmem_alloc(tmem_slot, kLTmemCols);
+    tmem_relinquish();
+  }
+  if (warp == 3) {
+    int seg = 0, row0 = 0;
+    const int rows = find_tile(p, blockIdx.x / C, lane, seg, row0);
+    if (lane == 0) {
+      tile_word[0] = rows;
+      tile_word[1] = seg;
+      tile_word[2] = row0;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  const int rows = tile_word[0], row0 = tile_word[2];
+  int adapter = rows > 0 ? p.seg_adapter[tile_word[1]] : -1;
+  if (adapter >= p.adapters) {
+    if (threadIdx.x == 0 && p.status) atomicCAS(p.status, 0, B200_LORA_STATUS_BAD_ADAPTER);
+    adapter = -1;
+  }
+  // This CTA's part of K and of N (the same for every tile)
+  const int nkb = (p.k + kTK - 1) / kTK, nnb = (p.n + kTN - 1) / kTN;
+  auto k_begin = [&](int c) { return static_cast<int>(static_cast<int64_t>(nkb) * c / C); };
+  const int nk = k_begin(rank + 1) - k_begin(rank);
+  const int n_first = static_cast<int>(static_cast<int64_t>(nnb) * rank / C);
+  const int nb = static_cast<int>(static_cast<int64_t>(nnb) * (rank + 1) / C) - n_first;
+
+  if (adapter < 0) {  // the whole cluster: nothing to add (rows of y are copied to out)
+    if (rows > 0 && p.out != p.y) {
+      const int c0 = n_first * kTN, c1 = min((n_first + nb) * kTN, p.n);
+      const int per = (c1 - c0) / 8;
+      for (int i = threadIdx.x; i < rows * per; i += kLThreads) {
+        const int64_t r = row0 + i / per, c = c0 + (i % per) * 8;
+        *reinterpret_cast<uint4*>(p.out + r * p.ldo + c) =
+            *reinterpret_cast<const uint4*>(p.y + r * p.ldy + c);
+      }
+    }
+    __syncthreads();
+    if (warp == 2) tmem_dealloc(tmem_base, kLTmemCols);
+    return;
+  }
+  if (C > 1) lora_cluster_sync();  // every CTA's barriers are ready for remote arrivals
+
+  const uint32_t a_bytes = p.rp * kTK * 2;
+  const uint32_t b_bytes = u_regions * kTN * kTK * 2;
+  // The partial sums, f32 [rp][128 rows], lie in the ring stages that step 3 fills last in
+  // its first round: stages (nk + NS - nx + i) % NS of a CTA with nk steps, per_stage
+  // columns in each.
+  const int per_stage = p.stage_bytes / (kTM * 4);
+  const int nx = C > 1 ? (p.rp + per_stage - 1) / per_stage : 0;
+  auto part_at = [&](int steps, int col) {  // this CTA's address of a column of partials
+    const int st = (steps + NS - nx + col / per_stage) % NS;
+    return reinterpret_cast<float*>(ring + st * p.stage_bytes) + (col % per_stage) * kTM;
+  };
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------ TMA producer
+    if (lane == 0) {
+      tma_prefetch_desc(&tm_x);
+      tma_prefetch_desc(&tm_a);
+      tma_prefetch_desc(&tm_b);
+      tma_prefetch_desc(&tm_y);
+      int it = 0;
+      bool ok = true;
+      const int kb0 = k_begin(rank);
+      for (; it < nk; ++it) {
+        const int s = it % NS;
+        if (!mbar_wait(empty + s, ((it / NS) & 1) ^ 1, abort_flag)) {
+          ok = false;
+          break;
+        }
+        uint8_t* dst = ring + s * p.stage_bytes;
+        mbar_expect_tx(full + s, kXBytes + a_bytes);
+        tma_load_2d(dst, &tm_x, full + s, (kb0 + it) * kTK, row0);
+        tma_load_3d(dst + kXBytes, &tm_a, full + s, (kb0 + it) * kTK, 0, adapter);
+      }
+      for (int i = 0; i < nb && ok; ++i, ++it) {
+        const int s = it % NS;
+        // first round: the stage's last use was in step 1; later: the epilogue has left it
+        ok = i < NS ? mbar_wait(empty + s, ((it / NS) & 1) ^ 1, abort_flag)
+                    : mbar_wait(empty2 + s, ((i / NS) & 1) ^ 1, abort_flag);
+        if (ok && i < NS && i >= NS - nx) ok = wait_cluster(slice_ready, 0, abort_flag);
+        if (!ok) break;
+        uint8_t* dst = ring + s * p.stage_bytes;
+        const int n0 = (n_first + i) * kTN;
+        mbar_expect_tx(full + s, kXBytes + b_bytes);
+        for (int r = 0; r < u_regions; ++r)
+          tma_load_3d(dst + kXBytes + r * kTN * kTK * 2, &tm_b, full + s, r * kTK, n0, adapter);
+        tma_load_2d(dst, &tm_y, full + s, n0, row0);
+      }
+      if (!ok) {
+        *abort_flag = 1;
+        if (p.status) atomicCAS(p.status, 0, 1);
+        for (int j = max(it - NS, 0); j < it; ++j)  // copies in flight land first
+          mbar_wait(full + j % NS, (j / NS) & 1);
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ MMA issuer
+    if (lane == 0) {
+      const uint32_t idesc_u = idesc_bf16_f32(kTM, p.rp, 0, 0);
+      constexpr uint32_t idesc_y = idesc_bf16_f32(kTM, kTN, 0, 0);
+      const uint64_t d0 = smem_desc(smem_addr(ring), 16, 1024);
+      const uint32_t hi = static_cast<uint32_t>(d0 >> 32), lo0 = static_cast<uint32_t>(d0);
+      const uint32_t lo_u = static_cast<uint32_t>(smem_desc(smem_addr(u_buf), 16, 1024));
+      bool ok = true;
+      int it = 0;
+      for (; it < nk; ++it) {
+        const int s = it % NS;
+        if (!mbar_wait(full + s, (it / NS) & 1, abort_flag)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t a = lo0 + ((s * p.stage_bytes) >> 4), b = a + (kXBytes >> 4);
+        mma_ss_off<0, 0>(tmem_base, a, hi, b, hi, idesc_u, it > 0 ? 1u : 0u);
+        mma_ss_off<2, 2>(tmem_base, a, hi, b, hi, idesc_u, 1u);
+        mma_ss_off<4, 4>(tmem_base, a, hi, b, hi, idesc_u, 1u);
+        mma_ss_off<6, 6>(tmem_base, a, hi, b, hi, idesc_u, 1u);
+        mma_commit(empty + s);
+      }
+      if (ok) mma_commit(u_full);
+      if (ok) ok = mbar_wait(u_ready, 0, abort_flag);
+      tc_fence_after();
+      for (int i = 0; i < nb && ok; ++i, ++it) {
+        const int s = it % NS;
+        if (!mbar_wait(full + s, (it / NS) & 1, abort_flag) ||
+            !mbar_wait(acc_empty + (i & 1), ((i >> 1) & 1) ^ 1, abort_flag)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t d = tmem_base + kAccCol + (i & 1) * kTN;
+        const uint32_t b = lo0 + ((s * p.stage_bytes + kXBytes) >> 4);
+        for (int kk = 0; kk < p.rp / 16; ++kk) {  // 16 of the rank: 32 bytes of the span
+          const uint32_t in = (kk & 3) * 2;
+          const uint32_t ao = lo_u + (kk >> 2) * (kXBytes >> 4) + in;
+          const uint32_t bo = b + (kk >> 2) * ((kTN * kTK * 2) >> 4) + in;
+          mma_ss_off<0, 0>(d, ao, hi, bo, hi, idesc_y, kk > 0 ? 1u : 0u);
+        }
+        mma_commit(acc_full + (i & 1));
+      }
+      if (!ok) {
+        *abort_flag = 1;
+        if (p.status) atomicCAS(p.status, 0, 2);
+      }
+    }
+  } else if (warp >= 4) {
+    // ------------------------------------------------------------------ epilogue
+    const int q = warp & 3;
+    const int tr = q * 32 + lane;  // row of the tile = TMEM lane
+    const uint32_t lane_off = static_cast<uint32_t>(q * 32) << 16;
+    const float scale = p.scale ? p.scale[adapter] : 1.f;
+    bool ok = mbar_wait(u_full, 0, abort_flag);
+    ok = __all_sync(0xffffffffu, ok);
+    tc_fence_after();
+    // u, 16 columns at a time; a CTA without any part of K has zeros
+    auto u_cols = [&](int c, uint32_t (&r)[16]) {
+      if (nk > 0) {
+        tmem_ld16(tmem_base + lane_off + c, r);
+        tmem_wait_ld();
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) r[i] = 0;
+      }
+    };
+    // 16-byte chunk j (8 of the rank) of row r in u_buf
+    auto u_chunk = [&](int r, int j) { return u_buf + (j >> 3) * kXBytes + r * 128 + (((j & 7) ^ (r & 7)) << 4); };
+    if (ok) {
+      if (C == 1) {
+        for (int c = 0; c < p.rp; c += 16) {
+          uint32_t r[16];
+          u_cols(c, r);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              w[e] = lora_pack(__uint_as_float(r[8 * j + 2 * e]) * scale, __uint_as_float(r[8 * j + 2 * e + 1]) * scale);
+            *reinterpret_cast<uint4*>(u_chunk(tr, c / 8 + j)) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+      } else {
+        for (int c = 0; c < p.rp; c += 16) {
+          uint32_t r[16];
+          u_cols(c, r);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) part_at(nk, c + i)[tr] = __uint_as_float(r[i]);
+        }
+        fence_proxy_async();  // the ring stages under the partials are TMA targets again later
+        epi_sync();
+        const int e = threadIdx.x - 128;
+        if (e < C) peer_arrive(part_ready, e);
+        ok = __all_sync(0xffffffffu, wait_cluster(part_ready, 0, abort_flag));
+        // this CTA's rows: 4 rows of one column at a time
+        const int rs = kTM / C;
+        for (int i = e; ok && i < p.rp * (rs / 4); i += 128) {
+          const int col = i / (rs / 4), r = rank * rs + (i % (rs / 4)) * 4;
+          float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int c = 0; c < C; ++c) {
+            const float4 v = peer_ld_f32x4(peer_addr(part_at(k_begin(c + 1) - k_begin(c), col) + r, c));
+            sum.x += v.x;
+            sum.y += v.y;
+            sum.z += v.z;
+            sum.w += v.w;
+          }
+          const float s4[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+          for (int z = 0; z < 4; ++z)
+            reinterpret_cast<__nv_bfloat16*>(u_chunk(r + z, col >> 3))[col & 7] = __float2bfloat16_rn(s4[z] * scale);
+        }
+        epi_sync();
+        if (e < C) peer_arrive(slice_ready, e);
+        ok = __all_sync(0xffffffffu, ok && wait_cluster(slice_ready, 0, abort_flag));
+        const int chunks = p.rp / 8;
+        for (int i = e; ok && i < kTM * chunks; i += 128) {
+          const int r = i / chunks, j = i % chunks;
+          if (r / rs != rank)
+            *reinterpret_cast<uint4*>(u_chunk(r, j)) = peer_ld_16b(peer_addr(u_chunk(r, j), r / rs));
+        }
+      }
+    }
+    fence_proxy_async();
+    tc_fence_before();
+    mbar_arrive(u_ready);
+    int it = nk;
+    for (int i = 0; i < nb && ok; ++i, ++it) {
+      const int s = it % NS;
+      ok = mbar_wait(full + s, (it / NS) & 1, abort_flag) &&
+           mbar_wait(acc_full + (i & 1), (i >> 1) & 1, abort_flag);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tc_fence_after();
+      uint8_t* yt = ring + s * p.stage_bytes;
+      uint4* yrow = reinterpret_cast<uint4*>(yt + tr * 128);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        uint32_t r[32];
+        tmem_ld32(tmem_base + kAccCol + lane_off + (i & 1) * kTN + half * 32, r);
+        tmem_wait_ld();
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint4* at = yrow + ((half * 4 + j) ^ (tr & 7));
+          const uint4 v = *at;
+          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+          uint32_t o[4];
+#pragma unroll
+          for (int z = 0; z < 4; ++z)
+            o[z] = lora_pack(__uint_as_float(w[z] << 16) + __uint_as_float(r[8 * j + 2 * z]),
+                             __uint_as_float(w[z] & 0xffff0000u) + __uint_as_float(r[8 * j + 2 * z + 1]));
+          *at = make_uint4(o[0], o[1], o[2], o[3]);
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(acc_empty + (i & 1));
+      // this warp's 32 rows: 4 rows of 128 bytes per pass
+      const int col = (n_first + i) * kTN + (lane & 7) * 8;
+#pragma unroll
+      for (int pass = 0; pass < 8; ++pass) {
+        const int rr = q * 32 + pass * 4 + (lane >> 3);
+        const uint4 v = reinterpret_cast<const uint4*>(yt)[rr * 8 + ((lane & 7) ^ (rr & 7))];
+        if (rr < rows && col < p.n)
+          *reinterpret_cast<uint4*>(p.out + static_cast<int64_t>(row0 + rr) * p.ldo + col) = v;
+      }
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(empty2 + s);
+    }
+    if (!ok && lane == 0) {
+      *abort_flag = 1;
+      if (p.status) atomicCAS(p.status, 0, 3);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (C > 1) lora_cluster_sync();  // peers may still read this CTA's rows of u
+  if (warp == 2) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, kLTmemCols);
+  }
+}
+
+// ------------------------------------------------------------------ host
+PFN_cuTensorMapEncodeTiled_v12000 lora_encode_fn() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q{};
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
+  });
+  return fn;
+}
+
+// bf16 map of [d2][d1][d0] (d0 dense, rows ld1 elements apart, planes ld2) with a box of
+// 64 x box1, 128-byte swizzle, zeros outside.  dims 2 or 3.
+int lora_map(CUtensorMap* map, const void* base, int dims, int64_t d0, int64_t d1, int64_t d2, int64_t ld1,
+             int64_t ld2, uint32_t box1) {
+  auto fn = lora_encode_fn();
+  if (!fn) return B200_ERR_CUDA;
+  const cuuint64_t size[3] = {static_cast<cuuint64_t>(d0), static_cast<cuuint64_t>(d1),
+                              static_cast<cuuint64_t>(d2)};
+  const cuuint64_t stride[2] = {static_cast<cuuint64_t>(ld1) * 2, static_cast<cuuint64_t>(ld2) * 2};
+  const cuuint32_t box[3] = {kTK, box1, 1};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, dims, const_cast<void*>(base), size, stride, box, estr,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+             ? B200_OK
+             : B200_ERR_CUDA;
+}
+
+int lora_sms() {
+  int dev = 0, n = 148;
+  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+  return n;
+}
+
+bool lora_al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+}  // namespace
+}  // namespace b200
+
+using namespace b200;
+
+extern "C" int b200_lora_add(const void* x, int64_t ldx, const void* a, const void* b, const void* y,
+                             int64_t ldy, void* out, int64_t ldo, const int32_t* seg_start,
+                             const int32_t* seg_adapter, const float* scale, int32_t rows,
+                             int32_t segments, int32_t adapters, int32_t n, int32_t k, int32_t rank,
+                             int32_t* status, b200_stream_t stream) {
+  if (rows < 0 || segments < 0 || adapters < 0 || n < 0) return B200_ERR_INVALID;
+  if (k <= 0 || k % 8 != 0 || n % 8 != 0 || rank <= 0 || rank % 8 != 0 || rank > B200_LORA_MAX_RANK)
+    return B200_ERR_INVALID;
+  if (rows == 0 || segments == 0 || n == 0) return B200_OK;
+  if (!x || !y || !out || !seg_start || !seg_adapter || (adapters > 0 && (!a || !b)))
+    return B200_ERR_INVALID;
+  const void* ptrs[] = {x, a, b, y, out};
+  for (const void* ptr : ptrs)
+    if (!lora_al16(ptr)) return B200_ERR_INVALID;
+  if (ldx < k || ldy < n || ldo < n || ldx % 8 != 0 || ldy % 8 != 0 || ldo % 8 != 0) return B200_ERR_INVALID;
+  if (out == y && ldo != ldy) return B200_ERR_INVALID;
+  LoraParams p{};
+  p.y = static_cast<const __nv_bfloat16*>(y);
+  p.out = static_cast<__nv_bfloat16*>(out);
+  p.ldy = ldy;
+  p.ldo = ldo;
+  p.seg_start = seg_start;
+  p.seg_adapter = seg_adapter;
+  p.scale = scale;
+  p.rows = rows;
+  p.segments = segments;
+  p.adapters = adapters;
+  p.n = n;
+  p.k = k;
+  p.rank = rank;
+  p.rp = (rank + 15) / 16 * 16;
+  p.status = status;
+  const int regions = p.rp > 64 ? 2 : 1;
+  p.stages = 3 + (regions - 1);
+  p.stage_bytes = kXBytes + regions * kTN * kTK * 2;
+  const int smem = p.stages * p.stage_bytes + regions * kXBytes + 256 + 1024;
+  // Every request ends in a tile of its own: rows / 128 + segments tiles at most.
+  const int64_t tiles = static_cast<int64_t>(rows) / kTM + std::min(segments, rows);
+  // Clusters of 1, 2, 4, 8 or 16 CTAs: enough CTAs for two per SM, a step of K and N each
+  const int64_t expect = std::max<int64_t>((rows + kTM - 1) / kTM, std::min(segments, rows));
+  const int steps = std::max((k + kTK - 1) / kTK, (n + kTN - 1) / kTN);
+  int C = 1;
+  while (C < 16 && expect * C * 2 <= 2 * lora_sms() && 2 * C <= steps) C *= 2;
+  p.C = C;
+  if (tiles * C > 0x7fffffff) return B200_ERR_INVALID;
+  CUtensorMap mx{}, ma{}, mb{}, my{};
+  int rc;
+  if ((rc = lora_map(&mx, x, 2, k, rows, 1, ldx, 0, kTM)) != B200_OK) return rc;
+  if ((rc = lora_map(&my, y, 2, n, rows, 1, ldy, 0, kTM)) != B200_OK) return rc;
+  if (adapters > 0) {
+    if ((rc = lora_map(&ma, a, 3, k, rank, adapters, k, static_cast<int64_t>(rank) * k, p.rp)) != B200_OK) return rc;
+    if ((rc = lora_map(&mb, b, 3, rank, n, adapters, rank, static_cast<int64_t>(rank) * n, kTN)) != B200_OK) return rc;
+  }
+  if (cudaFuncSetAttribute(lora_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
+      cudaFuncSetAttribute(lora_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
+    cudaGetLastError();
+    return B200_ERR_CUDA;
+  }
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(tiles * C));
+  cfg.blockDim = dim3(kLThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = C;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, lora_kernel, mx, ma, mb, my, p) != cudaSuccess) {
+    cudaGetLastError();
+    return B200_ERR_CUDA;
+  }
+  return cudaGetLastError() == cudaSuccess ? B200_OK : B200_ERR_CUDA;
+}

@@ -13,8 +13,8 @@ fn main() {
     let nvcc = env::var("NVCC").unwrap_or_else(|_| "nvcc".to_string());
     let arch = env::var("CUDA_ARCH_FLAGS")
         .unwrap_or_else(|_| "-gencode arch=compute_100a,code=sm_100a".to_string());
-    let sources = ["attn_fwd.cu", "block_ops.cu", "dequant.cu", "gemm.cu", "kv4.cu", "host_layout.cpp",
-                   "tp.cpp"];
+    let sources = ["attn_fwd.cu", "block_ops.cu", "dequant.cu", "gemm.cu", "kv4.cu", "lora.cu",
+                   "host_layout.cpp", "tp.cpp"];
     let mut cmd = Command::new(&nvcc);
     cmd.args(arch.split_whitespace())
         .args(["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC,-O3", "-shared",

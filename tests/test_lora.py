@@ -1,0 +1,159 @@
+"""Low-rank adapters of many requests beside a shared projection, against a plain 64-bit
+implementation.
+
+Tolerance per element: u = scale x A^T is summed in f32 (K terms, at most K 2^-24 of the sum
+of magnitudes), rounded to bf16 (2^-8), multiplied with B in f32, and the sum with y is
+rounded to bf16 (2^-8):
+|got - want| <= 2^-8 |want| + (2^-8 + 2^-10) * |scale| sum_r |u_r B_r|, where 2^-10 covers the
+f32 sums (K <= 12288: 12288 * 2^-24 = 2^-10.4 at the very most) and the second order."""
+import pytest
+import torch
+
+import b200attn
+
+
+def lib_call(rows=4, segments=2, adapters=3, n=64, k=64, rank=16, ldx=None, ldy=None, ldo=None, x=16, y=16,
+             out=32, a=16, b=16, seg=16, who=16):
+    return b200attn.lib().b200_lora_add(x, ldx or k, a, b, y, ldy or n, out, ldo or n, seg, who, None, rows,
+                                        segments, adapters, n, k, rank, None, None)
+
+
+def test_refuses_bad_arguments():
+    bad = b200attn.ERR_INVALID
+    for name in ("rows", "segments", "adapters", "n"):
+        assert lib_call(**{name: -1}) == bad
+    assert lib_call(k=0) == bad and lib_call(k=60) == bad and lib_call(n=60) == bad
+    assert lib_call(rank=0) == bad and lib_call(rank=12) == bad and lib_call(rank=136) == bad
+    assert lib_call(ldx=56) == bad and lib_call(ldy=56) == bad and lib_call(ldo=56) == bad
+    assert lib_call(ldx=68) == bad and lib_call(ldy=68) == bad and lib_call(ldo=68) == bad
+    for name in ("x", "y", "out", "a", "b", "seg", "who"):
+        assert lib_call(**{name: None}) == bad
+    for name in ("x", "y", "out", "a", "b"):
+        assert lib_call(**{name: 24}) == bad                  # not 16-byte aligned
+    assert lib_call(y=16, out=16, ldo=72) == bad              # in place with another stride
+    for name in ("rows", "segments", "n"):
+        assert lib_call(**{name: 0}) == b200attn.OK           # nothing to do, nothing launched
+
+
+def test_python_refuses_wrong_tensors():
+    bf = torch.bfloat16
+    x, y = torch.zeros(4, 64, dtype=bf), torch.zeros(4, 32, dtype=bf)
+    a, b = torch.zeros(2, 16, 64, dtype=bf), torch.zeros(2, 32, 16, dtype=bf)
+    seg, who = torch.tensor([0, 4], dtype=torch.int32), torch.tensor([0], dtype=torch.int32)
+    with pytest.raises(ValueError, match="CUDA"):
+        b200attn.lora_add(x, a, b, y, seg, who)
+    with pytest.raises(ValueError, match="x must be"):
+        b200attn.lora_add(x.float(), a, b, y, seg, who)
+    with pytest.raises(ValueError, match="b must have"):
+        b200attn.lora_add(x, a, b[:, :16], y, seg, who)
+    with pytest.raises(ValueError, match="seg_start"):
+        b200attn.lora_add(x, a, b, y, seg[:1], who)
+    with pytest.raises(ValueError, match="seg_adapter"):
+        b200attn.lora_add(x, a, b, y, seg, who.long())
+    with pytest.raises(ValueError, match="scale"):
+        b200attn.lora_add(x, a, b, y, seg, who, scale=torch.zeros(3))
+    with pytest.raises(ValueError, match="rows of y"):
+        b200attn.lora_add(x, a, b, y.t().contiguous().t(), seg, who)
+    with pytest.raises(ValueError, match="out must"):
+        b200attn.lora_add(x, a, b, y, seg, who, out=y[:3])
+
+
+def make(g, lens, who, k, n, rank, adapters, pad=0):
+    rows = sum(lens)
+    x = torch.randn(rows, k + pad, generator=g).bfloat16()[:, :k]
+    y = torch.randn(rows, n + pad, generator=g).bfloat16()[:, :n]
+    a = (torch.randn(adapters, rank, k, generator=g) * k ** -0.5).bfloat16()
+    b = torch.randn(adapters, n, rank, generator=g).bfloat16()
+    scale = torch.rand(adapters, generator=g) * 2 - 1
+    seg = torch.tensor([0] + torch.tensor(lens).cumsum(0).tolist(), dtype=torch.int32)
+    return x, y, a, b, scale, seg, torch.tensor(who, dtype=torch.int32)
+
+
+def check(got, x, y, a, b, scale, seg, who, before=None):
+    got = got.cpu().double()
+    want = (y if before is None else before).double().clone()
+    size = torch.zeros_like(want)
+    for s, e in enumerate(who.tolist()):
+        r = slice(int(seg[s]), int(seg[s + 1]))
+        if e < 0:
+            want[r] = y[r].double()
+            continue
+        f = 1.0 if scale is None else float(scale[e])
+        u = x[r].double() @ a[e].double().T
+        want[r] = y[r].double() + f * (u @ b[e].double().T)
+        size[r] = abs(f) * (u.abs() @ b[e].double().abs().T)
+    off = (got - want).abs()
+    assert (off <= 2 ** -8 * want.abs() + (2 ** -8 + 2 ** -10) * size).all(), off.max().item()
+
+
+CASES = [  # (rows of each request, adapters of them, K, N, rank, adapters)
+    ([1], [0], 64, 64, 16, 1),
+    ([1], [0], 8, 8, 8, 1),
+    ([1, 1, 1, 1], [2, 0, -1, 2], 4096, 4096, 16, 3),
+    ([3, 0, 128, 129, 1], [0, 1, 1, 0, 1], 200, 136, 8, 2),
+    ([127, 1, 128, 300], [1, -1, 0, 3], 1000, 520, 24, 4),
+    ([64] * 40, [i % 3 - 1 for i in range(40)], 512, 256, 64, 2),
+    ([1000], [0], 4096, 1024, 32, 1),
+    ([700, 5], [1, 0], 768, 4096, 128, 2),
+    ([2, 2], [0, 1], 136, 64, 72, 2),
+    ([2500, 2600, 17], [0, 1, 0], 256, 640, 48, 2),
+    ([40000], [0], 64, 72, 64, 1),
+    ([20000, 1], [0, 1], 72, 64, 128, 2),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens,who,k,n,rank,adapters", CASES)
+def test_lora_add(cuda, lens, who, k, n, rank, adapters):
+    g = torch.Generator().manual_seed(len(lens) * 1000 + k)
+    x, y, a, b, scale, seg, w = make(g, lens, who, k, n, rank, adapters)
+    dev = [t.to(cuda) for t in (x, a, b, y, seg, w)]
+    status = torch.zeros(1, dtype=torch.int32, device=cuda)
+    out = torch.full((sum(lens), n), 7.0, dtype=torch.bfloat16, device=cuda)
+    got = b200attn.lora_add(*dev, scale=scale.to(cuda), out=out, status=status)
+    assert got is out and status.item() == 0
+    check(got, x, y, a, b, scale, seg, w)
+    assert torch.equal(dev[3].cpu(), y)
+    again = b200attn.lora_add(*dev, scale=scale.to(cuda), out=torch.empty_like(out))
+    assert torch.equal(out, again)                            # sums in a fixed order
+    inplace = b200attn.lora_add(*dev, scale=scale.to(cuda))   # in place: the same bits
+    assert inplace is dev[3] and torch.equal(inplace, out)
+    assert status.item() == 0
+
+
+@pytest.mark.gpu
+def test_row_strides_gaps_and_foreign_rows(cuda):
+    """Rows wider than the operands, requests that leave rows out, NaN in the rows of others,
+    no scale, and the bytes around the rows left as they were."""
+    g = torch.Generator().manual_seed(5)
+    k, n, pad = 320, 200, 24
+    xf, yf = torch.randn(300, k + pad, generator=g).bfloat16(), torch.randn(300, n + pad, generator=g).bfloat16()
+    xf[100:110] = float("nan")
+    yf[100:110] = float("nan")
+    _, _, a, b, _, _, _ = make(g, [1], [0], k, n, 40, 2)
+    seg = torch.tensor([5, 100, 100, 110, 290], dtype=torch.int32)
+    who = torch.tensor([1, 0, -1, 0], dtype=torch.int32)
+    y_dev = yf.to(cuda)
+    b200attn.lora_add(xf.to(cuda)[:, :k], a.to(cuda), b.to(cuda), y_dev[:, :n], seg.to(cuda), who.to(cuda))
+    got = y_dev.cpu()
+    assert torch.equal(got[:, n:].nan_to_num(9), yf[:, n:].nan_to_num(9))
+    for r in (slice(0, 5), slice(290, 300), slice(100, 110)):
+        assert torch.equal(got[r].nan_to_num(9), yf[r].nan_to_num(9))
+    keep = [r for r in range(300) if not 100 <= r < 110]
+    ident = torch.tensor([5, 100, 280], dtype=torch.int32)
+    check(got[keep, :n], xf[keep, :k], yf[keep, :n], a, b, None, ident, torch.tensor([1, 0]), before=yf[keep, :n])
+
+
+@pytest.mark.gpu
+def test_bad_adapters_and_segments_stay_in_bounds(cuda):
+    """An adapter that is not there counts as none and is reported; starts outside the rows
+    are limited to them."""
+    g = torch.Generator().manual_seed(6)
+    x, y, a, b, scale, _, _ = make(g, [50], [0], 128, 64, 16, 2)
+    seg = torch.tensor([-20, 10, 30, 4000], dtype=torch.int32)
+    who = torch.tensor([0, 2, 1], dtype=torch.int32)
+    status = torch.zeros(1, dtype=torch.int32, device=cuda)
+    got = b200attn.lora_add(*(t.to(cuda) for t in (x, a, b, y, seg, who)), scale=scale.to(cuda),
+                            out=torch.zeros(50, 64, dtype=torch.bfloat16, device=cuda), status=status)
+    assert status.item() == b200attn.LORA_STATUS_BAD_ADAPTER
+    check(got, x, y, a, b, scale, torch.tensor([0, 10, 30, 50]), torch.tensor([0, -1, 1]))
