@@ -32,6 +32,7 @@ constexpr int kVsOff = 8704;   // V steps
 constexpr int kOctetBytes = 512;      // numbers of 8 tokens
 constexpr int kOctetStepBytes = 64;   // steps of 8 tokens
 constexpr float kTiny = 7.888609052210118e-31f;  // 2^-100
+constexpr float kHuge = 8.507059173023462e37f;   // 2^126: 24 steps of a group stay finite
 
 __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
   return __byte_perm(a, b, sel);
@@ -49,23 +50,43 @@ __device__ __forceinline__ void report_bad_page(int32_t* status) {
   if (status) atomicCAS(status, 0, B200_KV4_STATUS_BAD_PAGE);
 }
 
-// Nibbles i and i + 4 of w, each n + 8, as the bf16 pair (n, n): 0x4300 | u is the bf16
-// number 128 + u (7 mantissa bits, one unit each), and 128 + u - 136 = n is exact.
-__device__ __forceinline__ uint32_t nibble_pair(uint32_t w, int i) {
-  const uint32_t u = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
-  __nv_bfloat162 v = *reinterpret_cast<const __nv_bfloat162*>(&u);
-  const uint32_t bias = 0x43084308u;  // (136, 136)
-  v = __hsub2(v, *reinterpret_cast<const __nv_bfloat162*>(&bias));
-  return *reinterpret_cast<uint32_t*>(&v);
+// Nibbles i and i + 4 of w, each n + 8, as the bf16 pair 16 + u: u in the upper mantissa
+// bits.  One three-input operation for the mask and the exponent (left to itself the
+// compiler takes two, each with an immediate), and the shift to the left as a multiply,
+// which keeps off the ALU pipe: that pipe bounds the expansion.
+__device__ __forceinline__ uint32_t raw_pair(uint32_t w, int i) {
+  const uint32_t at = i == 0 ? w * 8u : w >> (4 * i - 3);
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(at), "r"(0x00780078u), "r"(0x41804180u));
+  return r;
+}
+
+// Nibbles i and i + 4 of w, each n + 8, times their steps: (16 + u) s - 24 s = n s in one packed
+// fma.  The
+// fma is exact: 24 s has at most 7 significant bits (s has 5) and n s has 8, so `less` =
+// -24 s and the result are bf16 numbers.  A step of 0 gives 0, NaN gives NaN.
+__device__ __forceinline__ uint32_t expand_pair(uint32_t w, int i, uint32_t step2, uint32_t less2) {
+  const uint32_t v = raw_pair(w, i);
+  const __nv_bfloat162 r = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&v),
+                                   *reinterpret_cast<const __nv_bfloat162*>(&step2),
+                                   *reinterpret_cast<const __nv_bfloat162*>(&less2));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+__device__ __forceinline__ uint32_t less_of(uint32_t step2) {  // -24 s, exact
+  const uint32_t k = 0xc1c0c1c0u;
+  const __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&step2),
+                                   *reinterpret_cast<const __nv_bfloat162*>(&k));
+  return *reinterpret_cast<const uint32_t*>(&r);
 }
 
 // ------------------------------------------------------------------ store
 // The step of a group whose largest magnitude is `top` (a bf16 value, or NaN): top / 7 cut
 // to 5 significant bits.  top has 8 bits, so the rounded quotient lies on its own side of
-// every 5-bit number.  Cutting, not rounding: 7 s <= top cannot overflow, and top / s < 7.44
-// still has the number 7.
+// every 5-bit number.  Cutting, not rounding: 7 s <= top, and top / s < 7.44 still has
+// the number 7.
 __device__ __forceinline__ float group_step(float top) {
-  if (!(top <= 3.402823466e38f)) return __uint_as_float(0x7fc00000u);  // infinity or NaN
+  if (!(top < kHuge)) return __uint_as_float(0x7fc00000u);  // infinity, NaN, or too large
   if (top < kTiny) return 0.f;
   return __uint_as_float(__float_as_uint(__fdiv_rn(top, 7.f)) & 0xfff80000u);
 }
@@ -225,14 +246,6 @@ struct LoadParams {
   int32_t* status;
 };
 
-// s * n of a nibble pair, exact in bf16.  A step that is zero keeps zeros, NaN gives NaN.
-__device__ __forceinline__ uint32_t scaled(uint32_t pair, uint32_t step2) {
-  const __nv_bfloat162 a = *reinterpret_cast<const __nv_bfloat162*>(&pair);
-  const __nv_bfloat162 s = *reinterpret_cast<const __nv_bfloat162*>(&step2);
-  const __nv_bfloat162 r = __hmul2(a, s);
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
-
 // grid (page, head, batch row), lanes as in the store.
 __global__ void __launch_bounds__(128) kv4_load_kernel(const LoadParams p) {
   const int b = blockIdx.z, h = blockIdx.y;
@@ -269,10 +282,10 @@ __global__ void __launch_bounds__(128) kv4_load_kernel(const LoadParams p) {
       const bool live = block && base + rk < len;
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        const uint32_t s2 = prmt(kss[c], kss[c], (g & 1) ? 0x3232 : 0x1010);
+        const uint32_t s2 = prmt(kss[c], kss[c], (g & 1) ? 0x3232 : 0x1010), less = less_of(s2);
         uint32_t pr[4];  // channels (i, i + 4)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) pr[i] = scaled(nibble_pair(kws[c], i), s2);
+        for (int i = 0; i < 4; ++i) pr[i] = expand_pair(kws[c], i, s2, less);
         const uint4 out = make_uint4(prmt(pr[0], pr[1], 0x5410), prmt(pr[2], pr[3], 0x5410),
                                      prmt(pr[0], pr[1], 0x7632), prmt(pr[2], pr[3], 0x7632));
         *reinterpret_cast<uint4*>(p.k + (row0 + rk) * kHeadDim + 32 * c + 8 * t) =
@@ -281,9 +294,10 @@ __global__ void __launch_bounds__(128) kv4_load_kernel(const LoadParams p) {
     }
 #pragma unroll
     for (int c = 0; c < 4; ++c) {  // V: tokens 2t, 2t + 1, pairs (token, token + 1)
+      const uint32_t less = less_of(vss[c]);
       uint32_t pr[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) pr[i] = scaled(nibble_pair(vws[c], i), vss[c]);
+      for (int i = 0; i < 4; ++i) pr[i] = expand_pair(vws[c], i, vss[c], less);
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
         const int rv = 8 * o + 2 * t + q;
@@ -322,22 +336,23 @@ __global__ void __launch_bounds__(256) kv4_copy_kernel(const __grid_constant__ C
 }
 
 // ------------------------------------------------------------------ attention of few rows
-// One cluster of S CTAs per (batch row, head, 16 query rows); the CTAs split the prefix's
-// pages, the 4 warps of a CTA split a page's 64 tokens, each warp with a running maximum m,
+// One cluster of S CTAs per (batch row, head, 8 J query rows); the CTAs split the prefix's
+// pages, the 2 warps of a CTA split a page's 64 tokens, each warp with a running maximum m,
 // sum l and unnormalised output of its own, joined at the end over the warps in shared
 // memory and over the CTAs through distributed shared memory, in a fixed order: no
 // workspace, no second launch, no atomics.
 //
-// Per page one 9216-byte bulk copy into a 4-deep ring (the block is contiguous); the ring
-// of 3 CTAs per SM keeps about 80 KB in flight.  Products run on mma m16n8k16 (bf16, f32
-// sums): at 1 to 16 rows the kernel is bound by the cache's bytes and by the instructions
-// that expand them, and a tcgen05 tile would need the numbers written to shared memory
-// again.  The numbers enter the products as the integers -7..7, exact in bf16:
-//   score_j = scale * sum over groups c of  kstep_jc * (q_c . n_jc)
-//   o_ch    = sum_j bf16(p_j * vstep_jc) * n_j,ch
-// so K's expansion rounds nothing, and V's rounds p once per group as the dense path
-// rounds p.  Channels are permuted alike in Q and K (and in V and the output), so that a
-// lane takes its fragments with one 16-byte shared load per octet.
+// A page and head is one contiguous block: one 9216-byte bulk copy per page into a ring.
+// Products run on mma m16n8k16 (bf16, f32 sums) with the keys (or V's channels) as the 16
+// rows and 8 queries as the columns: the expanded cache is the A operand, which takes the
+// whole of a warp's lanes even for one query, is expanded once for all J query tiles, and
+// costs half the instructions of the form with queries as rows.  The kernel is bound by the
+// instructions that expand the numbers: per 16 keys a warp issues about 260, and 4 warps
+// schedulers at HBM rate have 400 slots.  (A tcgen05 tile would need the expanded values
+// written to shared memory again.)
+//   S^T = K Q^T   K's values s * n are exact in bf16;
+//   O^T = V^T P^T V's too, P is rounded to bf16 as in the dense path; P^T comes out of S^T
+//                 by two 8x8 transposes (movmatrix).
 struct AttnParams4 {
   const uint8_t* pool;
   const int32_t* table;
@@ -351,17 +366,46 @@ struct AttnParams4 {
   float scale_log2;
 };
 
-constexpr int kRows = 16;        // query rows of a CTA
-constexpr int kRing = 4;
-constexpr int kAttnThreads = 128;
+constexpr int kMaxSplits = 8;
+constexpr int kWarps = 2;                // of a CTA
+constexpr int kThreads = 32 * kWarps;
+constexpr int kChunks = 4 / kWarps;      // 16-key chunks of a page per warp
+
+// J query tiles of 8 rows: a tile takes 32 registers for the output and 16 for Q.  A warp
+// takes 32 keys of a page at a time: two independent chains of products hide each other's
+// latency.  (4 warps of 16 keys, at as many warps per SM: 0.32 us per page and SM instead of
+// 0.28 for J = 1.  J = 4 takes 0.71 against 2 * 0.38 of J = 2, and fills its rows less often.)
+template <int J>
+struct AttnShape {
+  static constexpr int kRows = 8 * J;
+  static constexpr int kRing = J == 1 ? 3 : 4;
+  static constexpr int kCtas = J == 1 ? 8 : 6;                 // per SM, by registers
+  static constexpr int kJoin = kWarps * kRows * kHeadDim * 4;  // the warps' outputs
+  static constexpr int kUsed = kJoin + kRows * kHeadDim * 4;   // and the CTA's
+  static constexpr int kSmem = kRing * kBlock > kUsed ? kRing * kBlock : kUsed;
+};
+
+// d = a b + c
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                          uint32_t b1, const float (&c)[4]) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%10,%11,%12,%13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]),
+        "f"(c[3]));
+}
 
 __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
                                           uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-      "{%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  mma_16816(d, a, b0, b1, d);
+}
+
+// 8x8 transpose of 16-bit values: lane 4g + t gives row g, columns 2t, 2t + 1 and gets row
+// g of the transpose.
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
 }
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -374,16 +418,34 @@ __device__ __forceinline__ void cluster_barrier() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// The shared-memory word at `addr` of CTA `rank` of the cluster.
-__device__ __forceinline__ float remote_f32(const float* addr, uint32_t rank) {
-  float v;
-  asm volatile(
-      "{\n\t.reg .b32 ra;\n\tmapa.shared::cluster.u32 ra, %1, %2;\n\t"
-      "ld.shared::cluster.f32 %0, [ra];\n\t}"
-      : "=f"(v)
-      : "r"(smem_addr(addr)), "r"(rank)
-      : "memory");
+// Shared memory of CTA `rank` of the cluster, at this CTA's address `p`.
+__device__ __forceinline__ uint32_t peer_of(const void* p, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_addr(p)), "r"(rank));
+  return r;
+}
+
+__device__ __forceinline__ float2 peer_f32x2(uint32_t at) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory");
   return v;
+}
+
+__device__ __forceinline__ float4 peer_f32x4(uint32_t at) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(at)
+               : "memory");
+  return v;
+}
+
+// A whole warp waits: one try, which nearly always succeeds, and the bounded wait out of line.
+__device__ __noinline__ bool warp_wait_slow(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
+}
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  return __all_sync(0xffffffffu, mbar_try_wait(bar, parity)) || warp_wait_slow(bar, parity, abort_flag);
 }
 
 // 8 channels (one uint4) as the 4 pairs (j, j + 4) of the permuted order.
@@ -394,80 +456,93 @@ __device__ __forceinline__ void pairs_of(const uint4& u, uint32_t (&pr)[4]) {
   pr[3] = prmt(u.y, u.w, 0x7632);
 }
 
-__device__ __forceinline__ float quad_max(float v) {
-  v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
-  return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
-}
-
-__device__ __forceinline__ float quad_sum(float v) {
-  v += __shfl_xor_sync(0xffffffffu, v, 1);
-  return v + __shfl_xor_sync(0xffffffffu, v, 2);
-}
-
-// A warp's softmax state: lane 4g + t holds rows g and g + 8; o[4c + i] is the output tile
-// whose column 2t + e is channel 32c + 8t + 4e + i.
+// A warp's softmax state.  Lane 4g + t holds queries 8j + 2t + e; o[2c + z][j][2y + e] is
+// channel 32c + 4g + 2z + y of that query.  m is the same in all lanes of a t, less is -m
+// (0 before the first key); l is this lane's share.
+template <int J>
 struct WarpState {
-  float m[2], l[2];
-  float o[16][4];
+  float m[J][2], less[J][2], l[J][2];
+  float o[8][J][4];
 };
 
-// 16 keys: s[a][2r + e] is the score (log2 units) of row g + 8r and key 8a + 2t + e, -inf
-// where masked; vstep[a][c] the V steps of keys 2t, 2t + 1 of octet a as a bf16 pair;
-// vpair(a, c, i) the V fragment of octet a, group c, channel i.
-template <typename VPair>
-__device__ __forceinline__ void softmax_pv(WarpState& st, float (&s)[2][4], const uint32_t (&vstep)[2][4],
-                                           VPair vpair) {
-  float p[2][4], ref[2], alpha[2];
-  bool moved = false;
+// N times 16 keys: s[n][j][2y + e] is the product of key 8y + g of chunk n with query 8j +
+// 2t + e, times `scale` (log2 units) the score; -inf where masked.  va(n, c, z, a): the V
+// fragment of channels 32c + 4g + 2z + {0, 1}.  The running maximum is raised only when some
+// score of the warp exceeds its query's by more than kSlack (nearly every step is spared the
+// shuffles), so p <= 2^kSlack.
+constexpr float kSlack = 8.f;
+template <int J, int N, typename VFrag>
+__device__ __forceinline__ void softmax_pv(WarpState<J>& st, float (&s)[N][J][4], float scale, VFrag va) {
+  bool above = false;
+  float mx[J][2];
 #pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    const float mx =
-        quad_max(fmaxf(fmaxf(s[0][2 * r], s[0][2 * r + 1]), fmaxf(s[1][2 * r], s[1][2 * r + 1])));
-    const float m = fmaxf(st.m[r], mx);
-    moved |= m != st.m[r];
-    ref[r] = m == -INFINITY ? 0.f : m;  // no key so far: 2^(-inf - 0) = 0, not NaN
-    alpha[r] = ex2_approx(st.m[r] - ref[r]);
-    st.m[r] = m;
+  for (int j = 0; j < J; ++j)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      mx[j][e] = fmaxf(s[0][j][e], s[0][j][2 + e]);
+#pragma unroll
+      for (int n = 1; n < N; ++n) mx[j][e] = fmaxf(mx[j][e], fmaxf(s[n][j][e], s[n][j][2 + e]));
+      above |= mx[j][e] * scale > st.m[j][e] + kSlack;
+    }
+  if (__any_sync(0xffffffffu, above)) {
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      float alpha[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float m = mx[j][e] * scale;
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        m = fmaxf(st.m[j][e], m);
+        alpha[e] = m == -INFINITY ? 1.f : ex2_approx(st.m[j][e] - m);  // no key so far
+        st.m[j][e] = m;
+        // before the first key: 2^(-inf - 0) = 0, not 2^(-inf + inf)
+        st.less[j][e] = m == -INFINITY ? 0.f : -m;
+        st.l[j][e] *= alpha[e];
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int z = 0; z < 4; ++z) st.o[i][j][z] *= alpha[z & 1];
+    }
   }
+  uint32_t pt[N][J][2];
 #pragma unroll
-  for (int a = 0; a < 2; ++a)
+  for (int n = 0; n < N; ++n)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) p[a][i] = ex2_approx(s[a][i] - ref[i >> 1]);
-  if (__any_sync(0xffffffffu, moved)) {
+    for (int j = 0; j < J; ++j) {
+      float p[4];
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) st.o[i][e] *= alpha[e >> 1];
-    st.l[0] *= alpha[0];
-    st.l[1] *= alpha[1];
-  }
-#pragma unroll
-  for (int r = 0; r < 2; ++r)
-    st.l[r] += (p[0][2 * r] + p[0][2 * r + 1]) + (p[1][2 * r] + p[1][2 * r + 1]);
-#pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    uint32_t a[4];
-#pragma unroll
-    for (int o = 0; o < 2; ++o) {
-      const float v0 = bf16_lo(vstep[o][c]), v1 = bf16_hi(vstep[o][c]);
-      a[2 * o] = bf16_pair(p[o][0] * v0, p[o][1] * v1);
-      a[2 * o + 1] = bf16_pair(p[o][2] * v0, p[o][3] * v1);
+      for (int z = 0; z < 4; ++z) p[z] = ex2_approx(fmaf(s[n][j][z], scale, st.less[j][z & 1]));
+      st.l[j][0] += p[0] + p[2];
+      st.l[j][1] += p[1] + p[3];
+      pt[n][j][0] = transpose8(bf16_pair(p[0], p[1]));
+      pt[n][j][1] = transpose8(bf16_pair(p[2], p[3]));
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) mma_16816(st.o[4 * c + i], a, vpair(0, c, i), vpair(1, c, i));
-  }
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+      for (int z = 0; z < 2; ++z) {
+        uint32_t a[4];
+        va(n, c, z, a);
+#pragma unroll
+        for (int j = 0; j < J; ++j) mma_16816(st.o[2 * c + z][j], a, pt[n][j][0], pt[n][j][1]);
+      }
 }
 
-__global__ void __launch_bounds__(kAttnThreads, 3) kv4_attn_kernel(const AttnParams4 p) {
-  // The ring; after the last page, the warps' outputs [4][16][128].
-  __shared__ __align__(128) uint8_t ring[kRing * kBlock];
-  __shared__ __align__(16) float cta_o[kRows * kHeadDim];
-  __shared__ float warp_ml[2][4][kRows];
-  __shared__ float cta_ml[2][kRows];
+template <int J>
+__global__ void __launch_bounds__(kThreads, AttnShape<J>::kCtas) kv4_attn_kernel(const AttnParams4 p) {
+  using Shape = AttnShape<J>;
+  constexpr int kRing = Shape::kRing, kRows = Shape::kRows;
+  extern __shared__ __align__(128) uint8_t ring[];
+  // after the last page: the warps' outputs [kWarps][kRows][128] and the CTA's [kRows][128]
+  float* cta_o = reinterpret_cast<float*>(ring + Shape::kJoin);
+  __shared__ float warp_ml[2][kWarps][kRows];
+  __shared__ __align__(8) float cta_ml[kRows][2];
   __shared__ __align__(8) uint64_t full[kRing], empty[kRing];
-  __shared__ int page_ok[kRing];
   __shared__ int abort_word;
-  static_assert(kRing * kBlock >= 4 * kRows * kHeadDim * 4, "the ring holds the warps' outputs");
   volatile int* abort_flag = &abort_word;
 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -490,7 +565,7 @@ __global__ void __launch_bounds__(kAttnThreads, 3) kv4_attn_kernel(const AttnPar
   if (threadIdx.x == 0) {
     for (int i = 0; i < kRing; ++i) {
       mbar_init(full + i, 1);
-      mbar_init(empty + i, 4);
+      mbar_init(empty + i, kWarps);
     }
     abort_word = 0;
     fence_barrier_init();
@@ -511,15 +586,19 @@ __global__ void __launch_bounds__(kAttnThreads, 3) kv4_attn_kernel(const AttnPar
       if (j + 32 + lane < np) ids_next = ids_of[j + 32 + lane];
     }
     const int page = __shfl_sync(0xffffffffu, ids, j & 31);
-    if (lane == 0) {
-      const int slot = j % kRing;
-      const bool ok = page >= 0 && page < p.num_pages;
-      page_ok[slot] = ok;
-      if (ok) {
+    const int slot = j % kRing;
+    if (page >= 0 && page < p.num_pages) {
+      if (lane == 0) {
         mbar_expect_tx(full + slot, kBlock);
         bulk_load(ring + slot * kBlock, p.pool + (static_cast<int64_t>(page) * p.heads + h) * kBlock,
                   kBlock, full + slot);
-      } else {
+      }
+    } else {  // no such page: steps of 0 make its tokens read as zeros
+      for (int i = lane; i < (kBlock - kKsOff) / 16; i += 32)
+        *reinterpret_cast<uint4*>(ring + slot * kBlock + kKsOff + i * 16) = make_uint4(0, 0, 0, 0);
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) {
         report_bad_page(p.status);
         mbar_arrive(full + slot);
       }
@@ -529,152 +608,179 @@ __global__ void __launch_bounds__(kAttnThreads, 3) kv4_attn_kernel(const AttnPar
   if (warp == 0)
     for (; issued < np && issued < kRing; ++issued) issue(issued);
 
-  // Q fragments: rows g and g + 8 (zeros behind the last row)
-  uint32_t qf[8][4];
+  // Q fragments: query 8j + g (zeros behind the last row), channel pairs in the permuted order
+  uint32_t qf[8][J][2];
   {
     const __nv_bfloat16* qb =
         p.q + ((static_cast<int64_t>(b) * p.heads + h) * p.tokens + row0) * kHeadDim + 8 * t;
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      uint32_t lo[4], hi[4];
-      const uint4 zero = make_uint4(0, 0, 0, 0);
-      pairs_of(g < nrows ? *reinterpret_cast<const uint4*>(qb + g * kHeadDim + 32 * c) : zero, lo);
-      pairs_of(g + 8 < nrows ? *reinterpret_cast<const uint4*>(qb + (g + 8) * kHeadDim + 32 * c) : zero, hi);
+    for (int j = 0; j < J; ++j)
 #pragma unroll
-      for (int z = 0; z < 2; ++z) {
-        qf[2 * c + z][0] = lo[2 * z];
-        qf[2 * c + z][1] = hi[2 * z];
-        qf[2 * c + z][2] = lo[2 * z + 1];
-        qf[2 * c + z][3] = hi[2 * z + 1];
+      for (int c = 0; c < 4; ++c) {
+        const uint4 x = 8 * j + g < nrows
+                            ? *reinterpret_cast<const uint4*>(qb + (8 * j + g) * kHeadDim + 32 * c)
+                            : make_uint4(0, 0, 0, 0);
+        uint32_t pr[4];
+        pairs_of(x, pr);
+        qf[2 * c][j][0] = pr[0];
+        qf[2 * c][j][1] = pr[1];
+        qf[2 * c + 1][j][0] = pr[2];
+        qf[2 * c + 1][j][1] = pr[3];
       }
-    }
   }
-  WarpState st;
-  st.m[0] = st.m[1] = -INFINITY;
-  st.l[0] = st.l[1] = 0.f;
+  WarpState<J> st;
 #pragma unroll
-  for (int i = 0; i < 16; ++i)
+  for (int j = 0; j < J; ++j) {
+    st.m[j][0] = st.m[j][1] = -INFINITY;
+    st.less[j][0] = st.less[j][1] = 0.f;
+    st.l[j][0] = st.l[j][1] = 0.f;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) st.o[i][e] = 0.f;
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int z = 0; z < 4; ++z) st.o[i][j][z] = 0.f;
+  }
 
   // ---- this call's own keys (bf16), 16 at a time, dealt out over CTAs and warps
   {
-    int lim[2] = {tv, tv};
-    int most = tv;
-    if (p.row_limit) {
-#pragma unroll
-      for (int r = 0; r < 2; ++r)
-        lim[r] = min(tv, max(p.row_limit[min(row0 + g + 8 * r, p.tokens - 1)], 0));
-      most = min(tv, max(p.row_limit[row0 + nrows - 1], 0));
-    }
+    const int most = p.row_limit ? min(tv, max(p.row_limit[row0 + nrows - 1], 0)) : tv;
     const int chunks = (most + 15) / 16;
     const __nv_bfloat16* kb = p.k + (static_cast<int64_t>(b) * p.heads + h) * p.tokens * kHeadDim;
     const __nv_bfloat16* vb = p.v + (static_cast<int64_t>(b) * p.tokens * p.heads + h) * kHeadDim;
     const int64_t v_st = static_cast<int64_t>(p.heads) * kHeadDim;
-    for (int ch = rank + S * warp; ch < chunks; ch += 4 * S) {
-      float s[2][4];
+    for (int ch = rank + S * warp; ch < chunks; ch += kWarps * S) {
+      float s[1][J][4];
 #pragma unroll
-      for (int a = 0; a < 2; ++a) {
-        const int key = ch * 16 + 8 * a + g;
-        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int j = 0; j < J; ++j)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t pr[4];
-          pairs_of(key < tv ? *reinterpret_cast<const uint4*>(kb + static_cast<int64_t>(key) * kHeadDim + 32 * c + 8 * t)
-                            : make_uint4(0, 0, 0, 0), pr);
-          mma_16816(acc, qf[2 * c], pr[0], pr[1]);
-          mma_16816(acc, qf[2 * c + 1], pr[2], pr[3]);
-        }
+        for (int z = 0; z < 4; ++z) s[0][j][z] = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int kk = ch * 16 + 8 * a + 2 * t + (i & 1);
-          s[a][i] = kk < lim[i >> 1] ? acc[i] * p.scale_log2 : -INFINITY;
+      for (int c = 0; c < 4; ++c) {
+        uint32_t lo[4], hi[4];
+        const int k0 = ch * 16 + g, k1 = k0 + 8;
+        const uint4 zero = make_uint4(0, 0, 0, 0);
+        pairs_of(k0 < tv ? *reinterpret_cast<const uint4*>(kb + static_cast<int64_t>(k0) * kHeadDim + 32 * c + 8 * t) : zero, lo);
+        pairs_of(k1 < tv ? *reinterpret_cast<const uint4*>(kb + static_cast<int64_t>(k1) * kHeadDim + 32 * c + 8 * t) : zero, hi);
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {
+          const uint32_t a[4] = {lo[2 * z], hi[2 * z], lo[2 * z + 1], hi[2 * z + 1]};
+#pragma unroll
+          for (int j = 0; j < J; ++j) mma_16816(s[0][j], a, qf[2 * c + z][j][0], qf[2 * c + z][j][1]);
         }
       }
-      const uint32_t one = 0x3f803f80u;
-      const uint32_t vstep[2][4] = {{one, one, one, one}, {one, one, one, one}};
-      uint2 vx[2][2][4];  // [octet][parity][group]: channels 32c + 4g + 0..3
 #pragma unroll
-      for (int a = 0; a < 2; ++a)
+      for (int j = 0; j < J; ++j)
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
+        for (int e = 0; e < 2; ++e) {
+          int lim = tv;
+          if (p.row_limit) lim = min(tv, max(p.row_limit[min(row0 + 8 * j + 2 * t + e, p.tokens - 1)], 0));
+          if (ch * 16 + g >= lim) s[0][j][e] = -INFINITY;
+          if (ch * 16 + g + 8 >= lim) s[0][j][2 + e] = -INFINITY;
+        }
+      softmax_pv<J, 1>(st, s, p.scale_log2, [&](int, int c, int z, uint32_t (&a)[4]) {
+        uint32_t x[4];  // keys 2t, 2t + 1 (and 8 more), channels 32c + 4g + 2z + {0, 1}
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const int kk = ch * 16 + 8 * a + 2 * t + e;
-            vx[a][e][c] = kk < tv ? *reinterpret_cast<const uint2*>(vb + kk * v_st + 32 * c + 4 * g)
-                                  : make_uint2(0, 0);
-          }
-      softmax_pv(st, s, vstep, [&](int a, int c, int i) {
-        const uint2 x0 = vx[a][0][c], x1 = vx[a][1][c];
-        return prmt(i < 2 ? x0.x : x0.y, i < 2 ? x1.x : x1.y, (i & 1) ? 0x7632 : 0x5410);
+        for (int i = 0; i < 4; ++i) {
+          const int kk = ch * 16 + (i >> 1) * 8 + 2 * t + (i & 1);
+          x[i] = kk < tv ? *reinterpret_cast<const uint32_t*>(vb + kk * v_st + 32 * c + 4 * g + 2 * z) : 0u;
+        }
+        a[0] = prmt(x[0], x[1], 0x5410);
+        a[1] = prmt(x[0], x[1], 0x7632);
+        a[2] = prmt(x[2], x[3], 0x5410);
+        a[3] = prmt(x[2], x[3], 0x7632);
       });
     }
   }
 
   // ---- the prefix's pages
+  const uint32_t key_sel = (g & 1) ? 0x3232 : 0x1010;  // token g's step of a pair, twice
   bool ok = true;
+  int slot = 0;
+  uint32_t parity = 0;
   for (int j = 0; j < np; ++j) {
-    const int slot = j % kRing;
-    ok = __all_sync(0xffffffffu, mbar_wait(full + slot, (j / kRing) & 1, abort_flag));
+    ok = warp_wait(full + slot, parity, abort_flag);
     if (!ok) break;
-    const uint8_t* blk = ring + slot * kBlock;
-    const bool good = page_ok[slot] != 0;
-    const int left = pv - (first + j) * kPage - warp * 16;  // valid keys from this chunk on
+    const int left = pv - (first + j) * kPage - warp * (16 * kChunks);  // valid keys from here on
     if (left > 0) {
-      float s[2][4];
-      uint32_t vstep[2][4];
-      uint4 vw[2];
+      // chunk n of this warp: octets 2n and 2n + 1 from `at` on
+      const uint8_t* at = ring + slot * kBlock + warp * (kChunks * 2 * kOctetBytes) + lane * 16;
+      const uint8_t* steps = ring + slot * kBlock + kKsOff + warp * (kChunks * 2 * kOctetStepBytes);
+      auto load = [](const uint8_t* x) { return *reinterpret_cast<const uint4*>(x); };
+      auto word = [](const uint4& u, int c) { return c == 0 ? u.x : c == 1 ? u.y : c == 2 ? u.z : u.w; };
+      float s[kChunks][J][4];
 #pragma unroll
-      for (int a = 0; a < 2; ++a) {
-        const int octet = 2 * warp + a;
-        const uint4 kw4 = *reinterpret_cast<const uint4*>(blk + octet * kOctetBytes + lane * 16);
-        uint4 ks4 = *reinterpret_cast<const uint4*>(blk + kKsOff + octet * kOctetStepBytes + t * 16);
-        uint4 vs4 = *reinterpret_cast<const uint4*>(blk + kVsOff + octet * kOctetStepBytes + t * 16);
-        vw[a] = *reinterpret_cast<const uint4*>(blk + kVOff + octet * kOctetBytes + lane * 16);
-        if (!good) ks4 = vs4 = make_uint4(0, 0, 0, 0);  // reads as zeros
-        const uint32_t kw[4] = {kw4.x, kw4.y, kw4.z, kw4.w};
-        const uint32_t ks[4] = {ks4.x, ks4.y, ks4.z, ks4.w};
-        vstep[a][0] = vs4.x;
-        vstep[a][1] = vs4.y;
-        vstep[a][2] = vs4.z;
-        vstep[a][3] = vs4.w;
+      for (int n = 0; n < kChunks; ++n) {
+        uint4 kw[2], ks[2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[a][i] = 0.f;
+        for (int y = 0; y < 2; ++y) {
+          kw[y] = load(at + (2 * n + y) * kOctetBytes);
+          ks[y] = load(steps + (2 * n + y) * kOctetStepBytes + (g >> 1) * 16);
+        }
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          float acc[4] = {0.f, 0.f, 0.f, 0.f};
-          mma_16816(acc, qf[2 * c], nibble_pair(kw[c], 0), nibble_pair(kw[c], 1));
-          mma_16816(acc, qf[2 * c + 1], nibble_pair(kw[c], 2), nibble_pair(kw[c], 3));
-          const float s0 = bf16_lo(ks[c]) * p.scale_log2, s1 = bf16_hi(ks[c]) * p.scale_log2;
-          s[a][0] = fmaf(acc[0], s0, s[a][0]);
-          s[a][1] = fmaf(acc[1], s1, s[a][1]);
-          s[a][2] = fmaf(acc[2], s0, s[a][2]);
-          s[a][3] = fmaf(acc[3], s1, s[a][3]);
+          const uint32_t w0 = word(kw[0], c), w1 = word(kw[1], c), p0 = word(ks[0], c), p1 = word(ks[1], c);
+          const uint32_t s0 = prmt(p0, p0, key_sel), s1 = prmt(p1, p1, key_sel);
+          const uint32_t l0 = less_of(s0), l1 = less_of(s1);
+#pragma unroll
+          for (int z = 0; z < 2; ++z) {
+            const uint32_t a[4] = {expand_pair(w0, 2 * z, s0, l0), expand_pair(w1, 2 * z, s1, l1),
+                                   expand_pair(w0, 2 * z + 1, s0, l0), expand_pair(w1, 2 * z + 1, s1, l1)};
+#pragma unroll
+            for (int i = 0; i < J; ++i) {
+              const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+              if (c == 0 && z == 0) mma_16816(s[n][i], a, qf[0][i][0], qf[0][i][1], zero);
+              else mma_16816(s[n][i], a, qf[2 * c + z][i][0], qf[2 * c + z][i][1]);
+            }
+          }
         }
       }
-      if (left < 16) {  // behind the last token: no score, and no V step that could be NaN
+      const bool whole = left >= 16 * kChunks;
+      if (!whole) {  // no score behind the last token
 #pragma unroll
-        for (int a = 0; a < 2; ++a)
+        for (int n = 0; n < kChunks; ++n)
 #pragma unroll
-          for (int e = 0; e < 2; ++e)
-            if (8 * a + 2 * t + e >= left) {
-              s[a][e] = s[a][2 + e] = -INFINITY;
+          for (int i = 0; i < J; ++i)
 #pragma unroll
-              for (int c = 0; c < 4; ++c) vstep[a][c] &= e ? 0x0000ffffu : 0xffff0000u;
-            }
+            for (int z = 0; z < 4; ++z)
+              if (16 * n + 8 * (z >> 1) + g >= left) s[n][i][z] = -INFINITY;
       }
-      softmax_pv(st, s, vstep, [&](int a, int c, int i) {
-        const uint32_t w = c == 0 ? vw[a].x : c == 1 ? vw[a].y : c == 2 ? vw[a].z : vw[a].w;
-        return nibble_pair(w, i);
+      uint4 vw[2], vs[2];
+      softmax_pv<J, kChunks>(st, s, p.scale_log2, [&](int n, int c, int z, uint32_t (&a)[4]) {
+        if (c == 0 && z == 0) {
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            vw[y] = load(at + kVOff + (2 * n + y) * kOctetBytes);
+            vs[y] = load(steps + (kVsOff - kKsOff) + (2 * n + y) * kOctetStepBytes + t * 16);
+            if (!whole) {  // nor a V step that could be NaN
+              const int key = 16 * n + 8 * y + 2 * t;
+              const uint32_t keep = (key < left ? 0x0000ffffu : 0u) | (key + 1 < left ? 0xffff0000u : 0u);
+              vs[y].x &= keep;
+              vs[y].y &= keep;
+              vs[y].z &= keep;
+              vs[y].w &= keep;
+            }
+          }
+        }
+        const uint32_t v0 = word(vw[0], c), v1 = word(vw[1], c);
+        const uint32_t s0 = word(vs[0], c), s1 = word(vs[1], c);
+        const uint32_t l0 = less_of(s0), l1 = less_of(s1);
+        a[0] = expand_pair(v0, 2 * z, s0, l0);
+        a[1] = expand_pair(v0, 2 * z + 1, s0, l0);
+        a[2] = expand_pair(v1, 2 * z, s1, l1);
+        a[3] = expand_pair(v1, 2 * z + 1, s1, l1);
       });
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(empty + slot);
     // refill the slot that the page before left, which every warp is done with or about to be
     if (warp == 0 && j > 0 && issued < np) {
-      ok = __all_sync(0xffffffffu, mbar_wait(empty + (j - 1) % kRing, ((j - 1) / kRing) & 1, abort_flag));
+      const int prev = slot == 0 ? kRing - 1 : slot - 1;
+      ok = warp_wait(empty + prev, slot == 0 ? parity ^ 1 : parity, abort_flag);
       if (!ok) break;
       issue(issued++);
+    }
+    if (++slot == kRing) {
+      slot = 0;
+      parity ^= 1;
     }
   }
   if (!ok) {
@@ -691,82 +797,92 @@ __global__ void __launch_bounds__(kAttnThreads, 3) kv4_attn_kernel(const AttnPar
   {
     float* wo = reinterpret_cast<float*>(ring) + warp * kRows * kHeadDim;
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const float l = quad_sum(st.l[r]);
-      if (t == 0) {
-        warp_ml[0][warp][g + 8 * r] = st.m[r];
-        warp_ml[1][warp][g + 8 * r] = l;
+    for (int j = 0; j < J; ++j)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int q = 8 * j + 2 * t + e;
+        float l = st.l[j][e];
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        if (g == 0) {
+          warp_ml[0][warp][q] = st.m[j][e];
+          warp_ml[1][warp][q] = l;
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          *reinterpret_cast<float4*>(wo + q * kHeadDim + 32 * c + 4 * g) =
+              make_float4(st.o[2 * c][j][e], st.o[2 * c][j][2 + e], st.o[2 * c + 1][j][e], st.o[2 * c + 1][j][2 + e]);
       }
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-          *reinterpret_cast<float4*>(wo + (g + 8 * r) * kHeadDim + 32 * c + 8 * t + 4 * e) =
-              make_float4(st.o[4 * c][2 * r + e], st.o[4 * c + 1][2 * r + e], st.o[4 * c + 2][2 * r + e],
-                          st.o[4 * c + 3][2 * r + e]);
-    }
   }
   __syncthreads();
-  const int row = threadIdx.x >> 3;
-  if (row < nrows) {
-    float m = -INFINITY, l = 0.f, w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) m = fmaxf(m, warp_ml[0][i][row]);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float mi = warp_ml[0][i][row];
-      w[i] = mi == -INFINITY ? 0.f : ex2_approx(mi - m);
-      // a warp whose scores were all NaN keeps m = -inf and l = NaN: that NaN has to stay
-      l += mi == -INFINITY ? warp_ml[1][i][row] : w[i] * warp_ml[1][i][row];
-    }
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int ch = (threadIdx.x & 7) * 4 + 32 * k;
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float4 x = *reinterpret_cast<const float4*>(
-            reinterpret_cast<const float*>(ring) + (i * kRows + row) * kHeadDim + ch);
-        acc.x = fmaf(w[i], x.x, acc.x);
-        acc.y = fmaf(w[i], x.y, acc.y);
-        acc.z = fmaf(w[i], x.z, acc.z);
-        acc.w = fmaf(w[i], x.w, acc.w);
-      }
-      *reinterpret_cast<float4*>(cta_o + row * kHeadDim + ch) = acc;
-    }
-    if ((threadIdx.x & 7) == 0) {
-      cta_ml[0][row] = m;
-      cta_ml[1][row] = l;
-    }
-  }
-  // ---- join the CTAs: rank r finishes channels [128 r / S, 128 (r + 1) / S) of every row
-  if (S > 1) cluster_barrier();
-  else __syncthreads();
-  if (row < nrows) {
+  for (int i = threadIdx.x; i < nrows * (kHeadDim / 4); i += kThreads) {
+    const int row = i / (kHeadDim / 4), ch = (i % (kHeadDim / 4)) * 4;
     float m = -INFINITY, l = 0.f;
-    for (int i = 0; i < S; ++i) m = fmaxf(m, S > 1 ? remote_f32(&cta_ml[0][row], i) : cta_ml[0][row]);
-    for (int i = 0; i < S; ++i) {
-      const float mi = S > 1 ? remote_f32(&cta_ml[0][row], i) : cta_ml[0][row];
-      const float li = S > 1 ? remote_f32(&cta_ml[1][row], i) : cta_ml[1][row];
-      l += mi == -INFINITY ? li : ex2_approx(mi - m) * li;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) m = fmaxf(m, warp_ml[0][w][row]);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      // m = -inf: no key, weight 0 — or scores that were all NaN, whose NaN in l has to stay
+      const float mw = warp_ml[0][w][row];
+      const float f = mw == -INFINITY ? 0.f : ex2_approx(mw - m);
+      l += mw == -INFINITY ? warp_ml[1][w][row] : f * warp_ml[1][w][row];
+      const float4 x = *reinterpret_cast<const float4*>(
+          reinterpret_cast<const float*>(ring) + (w * kRows + row) * kHeadDim + ch);
+      acc.x = fmaf(f, x.x, acc.x);
+      acc.y = fmaf(f, x.y, acc.y);
+      acc.z = fmaf(f, x.z, acc.z);
+      acc.w = fmaf(f, x.w, acc.w);
     }
-    const float inv = 1.f / l;  // no key: 0 * (1 / 0) = NaN
-    const int per = kRows / S;  // channels of this thread
-    __nv_bfloat16* dst =
-        p.out + ((static_cast<int64_t>(b) * p.tokens + row0 + row) * p.heads + h) * kHeadDim;
-    for (int k = 0; k < per; ++k) {
-      const int ch = rank * (kHeadDim / S) + (threadIdx.x & 7) + 8 * k;
-      float acc = 0.f;
-      for (int i = 0; i < S; ++i) {
-        const float mi = S > 1 ? remote_f32(&cta_ml[0][row], i) : cta_ml[0][row];
-        const float w = mi == -INFINITY ? 0.f : ex2_approx(mi - m);
-        const float x = S > 1 ? remote_f32(cta_o + row * kHeadDim + ch, i) : cta_o[row * kHeadDim + ch];
-        acc = fmaf(w, x, acc);
+    if (S == 1) {
+      const float inv = 1.f / l;  // no key: 0 * (1 / 0) = NaN
+      __nv_bfloat16* dst =
+          p.out + ((static_cast<int64_t>(b) * p.tokens + row0 + row) * p.heads + h) * kHeadDim + ch;
+      *reinterpret_cast<uint2*>(dst) =
+          make_uint2(bf16_pair(acc.x * inv, acc.y * inv), bf16_pair(acc.z * inv, acc.w * inv));
+    } else {
+      *reinterpret_cast<float4*>(cta_o + row * kHeadDim + ch) = acc;
+      if (ch == 0) {
+        cta_ml[row][0] = m;
+        cta_ml[row][1] = l;
       }
-      dst[ch] = __float2bfloat16_rn(acc * inv);
     }
   }
-  if (S > 1) cluster_barrier();  // no CTA leaves while another reads its shared memory
+  if (S == 1) return;
+  // ---- join the CTAs: rank r finishes channels [128 r / S, 128 (r + 1) / S) of every row
+  cluster_barrier();
+  const int per = kHeadDim / S / 4;  // of 4 channels each
+  for (int i = threadIdx.x; i < nrows * per; i += kThreads) {
+    const int row = i / per, ch = rank * (kHeadDim / S) + (i % per) * 4;
+    float2 ml[kMaxSplits];
+    float4 x[kMaxSplits];
+#pragma unroll
+    for (int r = 0; r < kMaxSplits; ++r) {
+      const int from = r < S ? r : rank;  // past the last CTA: anything, with weight 0
+      ml[r] = peer_f32x2(peer_of(&cta_ml[row][0], from));
+      x[r] = peer_f32x4(peer_of(cta_o + row * kHeadDim + ch, from));
+    }
+    float m = -INFINITY, l = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int r = 0; r < kMaxSplits; ++r)
+      if (r < S) m = fmaxf(m, ml[r].x);
+#pragma unroll
+    for (int r = 0; r < kMaxSplits; ++r)
+      if (r < S) {
+        const float f = ml[r].x == -INFINITY ? 0.f : ex2_approx(ml[r].x - m);
+        l += ml[r].x == -INFINITY ? ml[r].y : f * ml[r].y;
+        acc.x = fmaf(f, x[r].x, acc.x);
+        acc.y = fmaf(f, x[r].y, acc.y);
+        acc.z = fmaf(f, x[r].z, acc.z);
+        acc.w = fmaf(f, x[r].w, acc.w);
+      }
+    const float inv = 1.f / l;
+    *reinterpret_cast<uint2*>(
+        p.out + ((static_cast<int64_t>(b) * p.tokens + row0 + row) * p.heads + h) * kHeadDim + ch) =
+        make_uint2(bf16_pair(acc.x * inv, acc.y * inv), bf16_pair(acc.z * inv, acc.w * inv));
+  }
+  cluster_barrier();  // no CTA leaves while another reads its shared memory
 }
 
 bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -801,13 +917,43 @@ int sm_count() {
   return sms;
 }
 
-// CTAs that share one row tile's pages: enough that the launch fills the GPU (3 CTAs per
-// SM), at most 8 (a portable cluster), and no fewer than 2 pages each.
-int pick_splits(int64_t items, int prefix_len) {
+// CTAs that share one row tile's pages: as many as run at once with a page each, and no more
+// than kPagesPerCta pages for one, so that rows of very different lengths even out (16 rows
+// of 1.3k to 10.6k tokens, 32 heads: 215 us unsplit, 97 us by 4 and by 8); at most 8, a
+// portable cluster.
+constexpr int kPagesPerCta = 24;
+int pick_splits(int64_t items, int prefix_len, int resident) {
   const int pages = (prefix_len + kPage - 1) / kPage;
   int s = 1;
-  while (s < 8 && items * s < 3 * sm_count() && pages >= 4 * s) s *= 2;
+  while (s < kMaxSplits &&
+         ((2 * items * s <= static_cast<int64_t>(resident) * sm_count() && pages >= 2 * s) ||
+          pages > kPagesPerCta * s))
+    s *= 2;
   return s;
+}
+
+template <int J>
+int launch_few_rows_of(AttnParams4 p, int batch, cudaStream_t stream) {
+  using Shape = AttnShape<J>;
+  p.row_tiles = (p.tokens + Shape::kRows - 1) / Shape::kRows;
+  const int64_t items = static_cast<int64_t>(batch) * p.heads * p.row_tiles;
+  p.splits = pick_splits(items, p.prefix_len, Shape::kCtas);
+  if (items * p.splits > 0x7fffffff) return B200_ERR_INVALID;
+  static_assert(Shape::kSmem <= 47 * 1024, "no attribute needed");
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(items * p.splits));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = Shape::kSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = p.splits;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kv4_attn_kernel<J>, p);
+  return e == cudaSuccess && cudaGetLastError() == cudaSuccess ? B200_OK : B200_ERR_CUDA;
 }
 
 int launch_few_rows(const b200_kv4_view& c, const void* q, const void* k, const void* v, int batch,
@@ -829,24 +975,8 @@ int launch_few_rows(const b200_kv4_view& c, const void* q, const void* k, const 
   p.heads = heads;
   p.tokens = tokens;
   p.prefix_len = prefix_len;
-  p.row_tiles = (tokens + kRows - 1) / kRows;
   p.scale_log2 = scale * 1.4426950408889634f;
-  const int64_t items = static_cast<int64_t>(batch) * heads * p.row_tiles;
-  p.splits = pick_splits(items, prefix_len);
-  if (items * p.splits > 0x7fffffff) return B200_ERR_INVALID;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(items * p.splits));
-  cfg.blockDim = dim3(kAttnThreads);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = p.splits;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kv4_attn_kernel, p);
-  return e == cudaSuccess && cudaGetLastError() == cudaSuccess ? B200_OK : B200_ERR_CUDA;
+  return tokens <= 8 ? launch_few_rows_of<1>(p, batch, stream) : launch_few_rows_of<2>(p, batch, stream);
 }
 
 size_t round256(size_t x) { return (x + 255) / 256 * 256; }

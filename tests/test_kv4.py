@@ -17,7 +17,7 @@ import torch
 import b200attn
 
 D, PAGE, BLOCK = 128, 64, 9216
-TINY = 2.0 ** -100
+TINY, HUGE = 2.0 ** -100, 2.0 ** 126
 
 
 # ----------------------------------------------------------------- plain definition
@@ -28,7 +28,7 @@ def quantise(x):
     frac, power = torch.frexp(top / 7)
     step = torch.ldexp(torch.floor(frac * 32) / 32, power)
     step = torch.where(top < TINY, 0.0, step)
-    step = torch.where(torch.isfinite(top), step, math.nan)
+    step = torch.where(top < HUGE, step, math.nan)
     use = (step > 0)[..., None]
     num = torch.where(use, torch.sign(g) * torch.floor(g.abs() / step[..., None] + 0.5), 0.0)
     return num.reshape(x.shape), step
@@ -80,7 +80,7 @@ def test_block_layout_is_a_bijection():
 def test_every_value_is_a_bf16_number():
     g = torch.Generator().manual_seed(3)
     x = (torch.randn(4000, D, generator=g) * torch.exp(8 * torch.randn(4000, 1, generator=g))).bfloat16()
-    x[0, :32] = 3.3895e38  # bf16's largest: 7 steps must not exceed it
+    x[0, :32] = 8.4e37  # next to the largest magnitude that a group may have
     v = values(x)
     assert torch.equal(v, v.to(torch.bfloat16).double())
     num, step = quantise(x)
@@ -235,7 +235,7 @@ def test_stored_bytes_follow_the_layout(cuda):
     x[0, 0, 0, 0] = (torch.arange(D) % 29 - 14) * 0.25   # halves of the step 1/2
     x[0, 0, 0, 1, :32] = 0
     x[0, 0, 0, 2, 32:64] = 2.0 ** -110
-    x[1, 0, 1, 3, 64:96] = 3.3895e38
+    x[1, 0, 1, 3, 64:96] = 8.4e37
     b200attn.kv4_store(x[0].to(cuda), x[1].to(cuda), pool, table)
     blocks = pool[table[0, 0].item()].cpu().numpy()
     for part in range(2):
@@ -288,13 +288,14 @@ def test_store_then_load(cuda, starts, counts, tokens, heads):
 
 @pytest.mark.gpu
 def test_non_finite_groups_read_as_nan(cuda):
-    pool, table, g = paged(cuda, [3], 1)
-    x = torch.randn(1, 1, 3, D, generator=g).bfloat16()
-    x[0, 0, 0, 5], x[0, 0, 1, 40], x[0, 0, 2, 127] = math.inf, -math.inf, math.nan
+    pool, table, g = paged(cuda, [4], 1)
+    x = torch.randn(1, 1, 4, D, generator=g).bfloat16()
+    x[0, 0, 0, 5], x[0, 0, 1, 40], x[0, 0, 2, 127], x[0, 0, 3, 0] = math.inf, -math.inf, math.nan, 2.0 ** 126
     b200attn.kv4_store(x.to(cuda), x.to(cuda), pool, table)
-    for got in b200attn.kv4_load(pool, table, None, 3):
-        nan = torch.isnan(got.cpu()).reshape(3, 4, 32)
-        assert nan[0, 0].all() and nan[1, 1].all() and nan[2, 3].all() and nan.sum() == 96
+    for got in b200attn.kv4_load(pool, table, None, 4):
+        nan = torch.isnan(got.cpu()).reshape(4, 4, 32)
+        assert nan[0, 0].all() and nan[1, 1].all() and nan[2, 3].all() and nan[3, 0].all()
+        assert nan.sum() == 128
 
 
 @pytest.mark.gpu
