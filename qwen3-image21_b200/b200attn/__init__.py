@@ -593,15 +593,15 @@ def _expect(t, name: str, dtype, shape, device, dense: bool = True) -> None:
 class _Launch:
     """Makes t's device current and, where a stream is given, that stream: the library
     launches on the current device, and what is allocated meanwhile belongs to the stream
-    that the kernels run on."""
+    that the kernels run on.  Yields the stream's handle."""
+    __slots__ = ("within", "index")
 
     def __init__(self, t, stream):
         import torch
         if not t.is_cuda:
             raise ValueError("the library computes on CUDA tensors only")
-        self.within = []
-        if t.device.index != torch.cuda.current_device():
-            self.within.append(torch.cuda.device(t.device))
+        self.within = ()
+        self.index = t.get_device()
         if stream is not None:
             if not isinstance(stream, torch.cuda.Stream):
                 raw = _stream(stream)
@@ -609,12 +609,15 @@ class _Launch:
                           else torch.cuda.default_stream(t.device))
             if stream.device != t.device:
                 raise ValueError(f"the stream is on {stream.device}, the tensors on {t.device}")
-            self.within.append(torch.cuda.stream(stream))
+            self.within = (torch.cuda.device(t.device), torch.cuda.stream(stream))
+        elif self.index != torch._C._cuda_getDevice():
+            self.within = (torch.cuda.device(t.device),)
 
     def __enter__(self):
+        import torch
         for c in self.within:
             c.__enter__()
-        return _stream(None)
+        return torch._C._cuda_getCurrentRawStream(self.index)
 
     def __exit__(self, *exc):
         for c in reversed(self.within):
@@ -697,8 +700,9 @@ def kv4_joint_attention(q_rot, k_rot, v, pool, page_table, prefix_len: int, desc
         _expect(row_limit, "row_limit", torch.int32, (t,), dev)
     with _Launch(pool, stream) as st:
         if out is None:
-            out = torch.empty((b, t, h * d), dtype=bf, device=dev)
-        _expect(out, "out", bf, (b, t, h * d), dev)
+            out = q_rot.new_empty((b, t, h * d))
+        else:
+            _expect(out, "out", bf, (b, t, h * d), dev)
         if workspace is None and t >= KV4_DENSE_QUERIES:
             workspace = torch.empty(kv4_workspace_bytes(b, h, t, prefix_len), dtype=torch.uint8,
                                     device=dev)

@@ -82,21 +82,36 @@ __device__ __forceinline__ uint32_t less_of(uint32_t step2) {  // -24 s, exact
 
 // ------------------------------------------------------------------ store
 // The step of a group whose largest magnitude is `top` (a bf16 value, or NaN): top / 7 cut
-// to 5 significant bits.  top has 8 bits, so the rounded quotient lies on its own side of
-// every 5-bit number.  Cutting, not rounding: 7 s <= top, and top / s < 7.44 still has
-// the number 7.
+// to 5 significant bits.  Cutting, not rounding: 7 s <= top, and top / s < 7.44 still has the
+// number 7.  The factor is 1/7 rounded up by 2^-20: a quotient that is a 5-bit number does
+// not fall below it, and any other is at least 1/7 unit of the 8-bit top away from one.
 __device__ __forceinline__ float group_step(float top) {
   if (!(top < kHuge)) return __uint_as_float(0x7fc00000u);  // infinity, NaN, or too large
   if (top < kTiny) return 0.f;
-  return __uint_as_float(__float_as_uint(__fdiv_rn(top, 7.f)) & 0xfff80000u);
+  return __uint_as_float(__float_as_uint(top * (0.14285714285714285 * (1.0 + 0x1p-20))) & 0xfff80000u);
 }
 
-// n + 8 of x for a step s > 0 (inv = 1 / s): |x| / s differs from a half by 0 or by at least
-// 2^-10 (x has 8 significant bits, s has 5, n at most 3), and |x| * inv is off by less than
-// 2^-20, so 2^-12 added sends exact halves up and moves no other value across one.
-__device__ __forceinline__ uint32_t number(float x, float inv) {
-  const int n = __float2int_rd(fmaf(fabsf(x), inv, 0.5f + 0.000244140625f));
-  return static_cast<uint32_t>(x < 0.f ? 8 - n : 8 + n);
+// The factor that number4 takes for a step (0 for a step of 0 or NaN, whose numbers are 0).
+// |x| / s differs from a half by 0 or by at least 1/496 (x has 8 significant bits, s has 5,
+// n at most 3): 1 + 2^-13 sends exact halves away from zero and moves no other value (below
+// 7.44) across one.
+__device__ __forceinline__ float number_scale(float step) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(step));
+  return step > 0.f ? r * (1.f + 0x1p-13f) : 0.f;
+}
+
+// n + 8 of the 4 values of two bf16 pairs as 4 nibbles in the low half: x * scale + 8 is
+// rounded to an integer by adding 1.5 * 2^23, and the nibbles are put together in f32 (exact
+// below 2^24), which keeps the work on the FMA pipe.
+__device__ __forceinline__ uint32_t number4(uint32_t w0, uint32_t w1, float scale) {
+  constexpr float kRound = 12582912.f;
+  const float x[4] = {bf16_lo(w0), bf16_hi(w0), bf16_lo(w1), bf16_hi(w1)};
+  float n[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) n[i] = fmaf(x[i], scale, kRound + 8.f) - kRound;
+  const float all = fmaf(n[3], 4096.f, fmaf(n[2], 256.f, fmaf(n[1], 16.f, n[0])));
+  return __float_as_uint(all + 8388608.f);
 }
 
 // As bit patterns, magnitudes of bf16 values order like integers, with infinity above every
@@ -165,57 +180,49 @@ __global__ void __launch_bounds__(128) kv4_store_kernel(const StoreParams p) {
 #pragma unroll
   for (int o = 0; o < 2; ++o) {
     const int octet = 2 * warp + o;
-    // ---- K
+    // ---- K: two groups' maxima share a word in the shuffles
     uint32_t words[4];
     float step[4];
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const uint32_t w[4] = {kx[o][c].x, kx[o][c].y, kx[o][c].z, kx[o][c].w};
-      uint32_t m = mag_max(mag_max(mag_max(mag_max(0u, w[0]), w[1]), w[2]), w[3]);
-      m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, 1));
-      m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, 2));
-      step[c] = group_step(__uint_as_float(max(m & 0xffffu, m >> 16) << 16));
-      const bool use = step[c] > 0.f;
-      const float inv = use ? __fdiv_rn(1.f, step[c]) : 0.f;
-      uint32_t out = 0;
+    for (int c = 0; c < 4; c += 2) {
+      uint32_t m[2];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        out |= (use ? number(bf16_lo(w[j]), inv) : 8u) << (8 * j);
-        out |= (use ? number(bf16_hi(w[j]), inv) : 8u) << (8 * j + 4);
+      for (int z = 0; z < 2; ++z) {
+        const uint4 x = kx[o][c + z];
+        m[z] = mag_max(mag_max(mag_max(mag_max(0u, x.x), x.y), x.z), x.w);
       }
-      words[c] = out;
+      uint32_t both = __vmaxu2(prmt(m[0], m[1], 0x5410), prmt(m[0], m[1], 0x7632));
+      both = __vmaxu2(both, __shfl_xor_sync(0xffffffffu, both, 1));
+      both = __vmaxu2(both, __shfl_xor_sync(0xffffffffu, both, 2));
+#pragma unroll
+      for (int z = 0; z < 2; ++z) {
+        const uint4 x = kx[o][c + z];
+        step[c + z] = group_step(z ? bf16_hi(both) : bf16_lo(both));
+        const float f = number_scale(step[c + z]);
+        words[c + z] = prmt(number4(x.x, x.y, f), number4(x.z, x.w, f), 0x5410);
+      }
     }
     if (have(8 * o + g)) {
       *reinterpret_cast<uint4*>(block + octet * kOctetBytes + lane * 16) =
           make_uint4(words[0], words[1], words[2], words[3]);
       // lane t writes group t's step of token g = 2t' + parity
       const float s = t == 0 ? step[0] : t == 1 ? step[1] : t == 2 ? step[2] : step[3];
-      reinterpret_cast<__nv_bfloat16*>(block + kKsOff + octet * kOctetStepBytes)[(g >> 1) * 8 + 2 * t + (g & 1)] =
-          __float2bfloat16_rn(s);
+      reinterpret_cast<uint16_t*>(block + kKsOff + octet * kOctetStepBytes)[(g >> 1) * 8 + 2 * t + (g & 1)] =
+          static_cast<uint16_t>(__float_as_uint(s) >> 16);
     }
-    // ---- V
-    uint32_t vw[4] = {0, 0, 0, 0}, vs[4] = {0, 0, 0, 0};
+    // ---- V: the two tokens' maxima share a word
+    uint32_t vw[4], vs[4];
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const uint32_t w[2] = {vx[o][q][c].x, vx[o][q][c].y};
-        uint32_t m = mag_max(mag_max(0u, w[0]), w[1]);
-        m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, 4));
-        m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, 8));
-        m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, 16));
-        const float s = group_step(__uint_as_float(max(m & 0xffffu, m >> 16) << 16));
-        const bool use = s > 0.f;
-        const float inv = use ? __fdiv_rn(1.f, s) : 0.f;
-        uint32_t half = 0;
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          half |= (use ? number(bf16_lo(w[j]), inv) : 8u) << (8 * j);
-          half |= (use ? number(bf16_hi(w[j]), inv) : 8u) << (8 * j + 4);
-        }
-        vw[c] |= half << (16 * q);
-        vs[c] |= (__float_as_uint(s) >> 16) << (16 * q);
-      }
+    for (int c = 0; c < 4; ++c) {
+      const uint2 x0 = vx[o][0][c], x1 = vx[o][1][c];
+      const uint32_t m0 = mag_max(mag_max(0u, x0.x), x0.y), m1 = mag_max(mag_max(0u, x1.x), x1.y);
+      uint32_t both = __vmaxu2(prmt(m0, m1, 0x5410), prmt(m0, m1, 0x7632));
+      both = __vmaxu2(both, __shfl_xor_sync(0xffffffffu, both, 4));
+      both = __vmaxu2(both, __shfl_xor_sync(0xffffffffu, both, 8));
+      both = __vmaxu2(both, __shfl_xor_sync(0xffffffffu, both, 16));
+      const float s0 = group_step(bf16_lo(both)), s1 = group_step(bf16_hi(both));
+      vs[c] = prmt(__float_as_uint(s0), __float_as_uint(s1), 0x7632);
+      vw[c] = prmt(number4(x0.x, x0.y, number_scale(s0)), number4(x1.x, x1.y, number_scale(s1)), 0x5410);
     }
     const bool h0 = have(8 * o + 2 * t), h1 = have(8 * o + 2 * t + 1);
     uint8_t* vd = block + kVOff + octet * kOctetBytes + lane * 16;

@@ -245,6 +245,31 @@ def test_stored_bytes_follow_the_layout(cuda):
 
 
 @pytest.mark.gpu
+def test_numbers_at_every_border(cuda):
+    """Every 8-bit largest magnitude of a group (all 128 mantissas) with every mantissa of the
+    other values at the exponents where a number can be 1 to 7, both signs: the halves that
+    are exact and the values next to a border get the definition's numbers."""
+    mant = 1 + torch.arange(128).double() / 128
+    other = torch.cat([mant * 2.0 ** e for e in range(-5, 1)])           # 768 values up to 2
+    other = torch.cat([other, -other])
+    rows = []
+    for top in mant:
+        use = other[other.abs() <= top]
+        use = torch.nn.functional.pad(use, (0, -len(use) % 31))
+        part = use.reshape(-1, 31)
+        rows.append(torch.cat([torch.full((len(part), 1), float(top)), part.float()], 1))
+    x = torch.cat(rows)
+    x = torch.nn.functional.pad(x, (0, 0, 0, -len(x) % 4)).reshape(-1, D).bfloat16()
+    assert torch.equal(x.double().reshape(-1, 32)[:len(rows[0])], rows[0].double())
+    x = x.reshape(1, 1, -1, D)
+    n = x.shape[2]
+    pool, table, _ = paged(cuda, [n], 1)
+    b200attn.kv4_store(x.to(cuda), -x.to(cuda), pool, table)
+    k, v = b200attn.kv4_load(pool, table, None, n)
+    assert torch.equal(k.cpu().double(), values(x)) and torch.equal(v.cpu().double(), values(-x))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("starts,counts,tokens,heads", [
     ([0], [1], 1, 1), ([63], [2], 2, 3), ([0, 5, 64], [130, 1, 0], 130, 2),
     ([7, 200], [64, 3], 64, 4), ([15, 16, 17], [16, 15, 33], 33, 1), ([1], [511], 600, 5),
