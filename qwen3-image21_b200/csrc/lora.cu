@@ -8,7 +8,8 @@
 //   1. CTA c multiplies its part of K: x tiles [128 x 64] and A tiles [rank x 64] arrive by
 //      TMA, u_c accumulates in TMEM (tcgen05.mma M128 N=rank).
 //   2. The partial sums meet through distributed shared memory: CTA c adds the C partials of
-//      its 128 / C rows in rank order, scales, rounds to bf16, and fetches the other rows.
+//      its 128 / C rows in rank order, scales, rounds to bf16, and fetches the other rows
+//      (of few rows, each CTA adds up all).
 //   3. CTA c walks its part of N in 64-column steps: B tiles and y tiles by TMA, u B^T in
 //      TMEM (two accumulators), the epilogue adds y in shared memory and writes whole
 //      128-byte row segments.  Rows of another request in the tile are not written.
@@ -22,6 +23,7 @@
 #include <algorithm>
 #include <cstdint>
 #include <mutex>
+#include <type_traits>
 
 #include "../../include/b200_lora.h"
 #include "ptx.cuh"
@@ -37,6 +39,11 @@ constexpr int kLThreads = 256;
 constexpr uint32_t kLTmemCols = 256;     // u: 128 columns, two accumulators of 64
 constexpr uint32_t kAccCol = 128;
 constexpr int kMaxStages = 4;
+constexpr int kMaxC = 16;
+constexpr int kMaxExtent = 1 << 30;      // of K and N
+// Columns times groups of 4 rows of u up to which every CTA of a cluster adds the partials up
+// for itself, which saves one exchange between the CTAs.
+constexpr int kDirect = 256;
 
 struct LoraParams {
   const __nv_bfloat16* y;
@@ -48,7 +55,7 @@ struct LoraParams {
   int32_t rows, segments, adapters, n, k, rank;
   int32_t rp;            // rank rounded up to 16
   int32_t stages, stage_bytes;
-  int32_t C;             // CTAs of a cluster
+  int32_t C, log_c;      // CTAs of a cluster, a power of two
   int32_t* status;
 };
 
@@ -161,7 +168,25 @@ __device__ __forceinline__ int find_tile(const LoraParams& p, int tile, int lane
   return 0;
 }
 
-__global__ void __launch_bounds__(kLThreads)
+// Rows [row, row + 4) of one column of u: the C partials, loaded together (a remote load takes
+// about half a microsecond) and added in rank order.
+template <int C>
+__device__ __forceinline__ float4 sum_partials(const uint32_t (&at)[C]) {
+  float4 v[C];
+#pragma unroll
+  for (int c = 0; c < C; ++c) v[c] = peer_ld_f32x4(at[c]);
+  float4 sum = v[0];
+#pragma unroll
+  for (int c = 1; c < C; ++c) {
+    sum.x += v[c].x;
+    sum.y += v[c].y;
+    sum.z += v[c].z;
+    sum.w += v[c].w;
+  }
+  return sum;
+}
+
+__global__ void __launch_bounds__(kLThreads, 2)
     lora_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_a,
                 const __grid_constant__ CUtensorMap tm_b, const __grid_constant__ CUtensorMap tm_y,
                 const LoraParams p) {
@@ -232,10 +257,11 @@ __global__ void __launch_bounds__(kLThreads)
   }
   // This CTA's part of K and of N (the same for every tile)
   const int nkb = (p.k + kTK - 1) / kTK, nnb = (p.n + kTN - 1) / kTN;
-  auto k_begin = [&](int c) { return static_cast<int>(static_cast<int64_t>(nkb) * c / C); };
+  // (K, N <= 2^30: 16 times their steps of 64 stay in 32 bits)
+  auto k_begin = [&](int c) { return (nkb * c) >> p.log_c; };
   const int nk = k_begin(rank + 1) - k_begin(rank);
-  const int n_first = static_cast<int>(static_cast<int64_t>(nnb) * rank / C);
-  const int nb = static_cast<int>(static_cast<int64_t>(nnb) * (rank + 1) / C) - n_first;
+  const int n_first = (nnb * rank) >> p.log_c;
+  const int nb = ((nnb * (rank + 1)) >> p.log_c) - n_first;
 
   if (adapter < 0) {  // the whole cluster: nothing to add (rows of y are copied to out)
     if (rows > 0 && p.out != p.y) {
@@ -255,14 +281,17 @@ __global__ void __launch_bounds__(kLThreads)
 
   const uint32_t a_bytes = p.rp * kTK * 2;
   const uint32_t b_bytes = u_regions * kTN * kTK * 2;
-  // The partial sums, f32 [rp][128 rows], lie in the ring stages that step 3 fills last in
-  // its first round: stages (nk + NS - nx + i) % NS of a CTA with nk steps, per_stage
-  // columns in each.
+  // The partial sums, f32 [rp][128 rows], lie in the one or two ring stages that step 3
+  // fills last in its first round: stages (nk + NS - nx + i) % NS of a CTA with nk steps, with
+  // per_stage columns in each.
   const int per_stage = p.stage_bytes / (kTM * 4);
-  const int nx = C > 1 ? (p.rp + per_stage - 1) / per_stage : 0;
+  const int nx = C == 1 ? 0 : p.rp > per_stage ? 2 : 1;
+  const int steps0 = nkb >> p.log_c, stage0 = (steps0 + NS - nx) % NS;  // of a CTA with steps0
   auto part_at = [&](int steps, int col) {  // this CTA's address of a column of partials
-    const int st = (steps + NS - nx + col / per_stage) % NS;
-    return reinterpret_cast<float*>(ring + st * p.stage_bytes) + (col % per_stage) * kTM;
+    const int second = col >= per_stage ? 1 : 0;
+    int st = stage0 + (steps - steps0) + second;  // steps is steps0 or one more
+    if (st >= NS) st -= NS;
+    return reinterpret_cast<float*>(ring + st * p.stage_bytes) + (col - second * per_stage) * kTM;
   };
 
   if (warp == 0) {
@@ -404,31 +433,64 @@ __global__ void __launch_bounds__(kLThreads)
         const int e = threadIdx.x - 128;
         if (e < C) peer_arrive(part_ready, e);
         ok = __all_sync(0xffffffffu, wait_cluster(part_ready, 0, abort_flag));
-        // this CTA's rows: 4 rows of one column at a time
-        const int rs = kTM / C;
-        for (int i = e; ok && i < p.rp * (rs / 4); i += 128) {
-          const int col = i / (rs / 4), r = rank * rs + (i % (rs / 4)) * 4;
-          float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-          for (int c = 0; c < C; ++c) {
-            const float4 v = peer_ld_f32x4(peer_addr(part_at(k_begin(c + 1) - k_begin(c), col) + r, c));
-            sum.x += v.x;
-            sum.y += v.y;
-            sum.z += v.z;
-            sum.w += v.w;
-          }
-          const float s4[4] = {sum.x, sum.y, sum.z, sum.w};
+        // Sums of `quads` groups of 4 rows from row `from` on, one column of one group at a
+        // time: U of them in flight.
+        auto reduce = [&](auto c_tag, int from, int quads) {
+          constexpr int CC = decltype(c_tag)::value, U = CC >= 8 ? 1 : 8 / CC;
+          const int units = p.rp * quads;
+          for (int i0 = e; ok && i0 < units; i0 += 128 * U) {
+            float4 sum[U];
 #pragma unroll
-          for (int z = 0; z < 4; ++z)
-            reinterpret_cast<__nv_bfloat16*>(u_chunk(r + z, col >> 3))[col & 7] = __float2bfloat16_rn(s4[z] * scale);
-        }
-        epi_sync();
-        if (e < C) peer_arrive(slice_ready, e);
-        ok = __all_sync(0xffffffffu, ok && wait_cluster(slice_ready, 0, abort_flag));
-        const int chunks = p.rp / 8;
-        for (int i = e; ok && i < kTM * chunks; i += 128) {
-          const int r = i / chunks, j = i % chunks;
-          if (r / rs != rank)
-            *reinterpret_cast<uint4*>(u_chunk(r, j)) = peer_ld_16b(peer_addr(u_chunk(r, j), r / rs));
+            for (int u = 0; u < U; ++u) {
+              const int i = min(i0 + 128 * u, units - 1), col = i / quads, r = from + (i % quads) * 4;
+              uint32_t at[CC];
+#pragma unroll
+              for (int c = 0; c < CC; ++c)
+                at[c] = peer_addr(part_at(k_begin(c + 1) - k_begin(c), col) + r, c);
+              sum[u] = sum_partials<CC>(at);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+              const int i = i0 + 128 * u, col = i / quads, r = from + (i % quads) * 4;
+              if (i >= units) break;
+              const float s4[4] = {sum[u].x, sum[u].y, sum[u].z, sum[u].w};
+#pragma unroll
+              for (int z = 0; z < 4; ++z)
+                reinterpret_cast<__nv_bfloat16*>(u_chunk(r + z, col >> 3))[col & 7] =
+                    __float2bfloat16_rn(s4[z] * scale);
+            }
+          }
+        };
+        auto reduce_rows = [&](int from, int quads) {
+          if (C == 2) reduce(std::integral_constant<int, 2>(), from, quads);
+          else if (C == 4) reduce(std::integral_constant<int, 4>(), from, quads);
+          else if (C == 8) reduce(std::integral_constant<int, 8>(), from, quads);
+          else reduce(std::integral_constant<int, 16>(), from, quads);
+        };
+        const int rs = kTM / C, quads = (rows + 3) / 4;
+        if (quads * p.rp <= kDirect) {  // few rows: every CTA adds them all up for itself
+          reduce_rows(0, quads);
+          epi_sync();
+          if (e < C) peer_arrive(slice_ready, e);
+        } else {                        // its own share, then the others' from them
+          reduce_rows(rank * rs, rs / 4);
+          epi_sync();
+          if (e < C) peer_arrive(slice_ready, e);
+          ok = __all_sync(0xffffffffu, ok && wait_cluster(slice_ready, 0, abort_flag));
+          const int chunks = p.rp / 8, all = rows * chunks;
+          for (int i0 = e; ok && i0 < all; i0 += 128 * 4) {
+            uint4 v[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              const int i = min(i0 + 128 * u, all - 1), r = i / chunks;
+              v[u] = peer_ld_16b(peer_addr(u_chunk(r, i % chunks), r / rs));
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              const int i = i0 + 128 * u, r = i / chunks;
+              if (i < all && r / rs != rank) *reinterpret_cast<uint4*>(u_chunk(r, i % chunks)) = v[u];
+            }
+          }
         }
       }
     }
@@ -525,9 +587,44 @@ int lora_map(CUtensorMap* map, const void* base, int dims, int64_t d0, int64_t d
              : B200_ERR_CUDA;
 }
 
-int lora_sms() {
-  int dev = 0, n = 148;
-  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+int lora_attributes(int smem) {
+  if (cudaFuncSetAttribute(lora_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) == cudaSuccess &&
+      cudaFuncSetAttribute(lora_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess)
+    return B200_OK;
+  cudaGetLastError();
+  return B200_ERR_CUDA;
+}
+
+// Clusters of C CTAs that the current device runs at once (clusters do not straddle its GPU
+// clusters, so this is less than the CTAs that fit / C).  The occupancy query counts one CTA
+// per SM for a kernel with tensor memory; with its 256 of the SM's 512 columns, two run
+// wherever shared memory holds two.  A property of the kernel and the device, asked for once.
+constexpr int kTwoPerSm = 113 * 1024;  // dynamic shared memory of which an SM holds two
+int active_clusters(int C, int smem) {
+  static std::mutex lock;
+  static int known[64][2][kMaxC + 1] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+  std::lock_guard<std::mutex> hold(lock);
+  int& n = known[dev][smem > kTwoPerSm ? 1 : 0][C];
+  if (n == 0) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(C);
+    cfg.blockDim = dim3(kLThreads);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = C;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&n, lora_kernel, &cfg) != cudaSuccess) {
+      cudaGetLastError();
+      return 0;
+    }
+    if (smem <= kTwoPerSm) n *= 2;
+  }
   return n;
 }
 
@@ -544,7 +641,7 @@ extern "C" int b200_lora_add(const void* x, int64_t ldx, const void* a, const vo
                              int32_t segments, int32_t adapters, int32_t n, int32_t k, int32_t rank,
                              int32_t* status, b200_stream_t stream) {
   if (rows < 0 || segments < 0 || adapters < 0 || n < 0) return B200_ERR_INVALID;
-  if (k <= 0 || k % 8 != 0 || n % 8 != 0 || rank <= 0 || rank % 8 != 0 || rank > B200_LORA_MAX_RANK)
+  if (k <= 0 || k > kMaxExtent || n > kMaxExtent || k % 8 != 0 || n % 8 != 0 || rank <= 0 || rank % 8 != 0 || rank > B200_LORA_MAX_RANK)
     return B200_ERR_INVALID;
   if (rows == 0 || segments == 0 || n == 0) return B200_OK;
   if (!x || !y || !out || !seg_start || !seg_adapter || (adapters > 0 && (!a || !b)))
@@ -574,27 +671,29 @@ extern "C" int b200_lora_add(const void* x, int64_t ldx, const void* a, const vo
   p.stages = 3 + (regions - 1);
   p.stage_bytes = kXBytes + regions * kTN * kTK * 2;
   const int smem = p.stages * p.stage_bytes + regions * kXBytes + 256 + 1024;
-  // Every request ends in a tile of its own: rows / 128 + segments tiles at most.
+  // Every request ends in a tile of its own: rows / 128 + segments tiles at most.  The
+  // cluster is the largest whose tiles are expected to run all at once: with every request's
+  // last tile half full on average.
   const int64_t tiles = static_cast<int64_t>(rows) / kTM + std::min(segments, rows);
-  // Clusters of 1, 2, 4, 8 or 16 CTAs: enough CTAs for two per SM, a step of K and N each
-  const int64_t expect = std::max<int64_t>((rows + kTM - 1) / kTM, std::min(segments, rows));
+  const int64_t expect = std::min<int64_t>(tiles, (rows + kTM - 1) / kTM + segments / 2);
   const int steps = std::max((k + kTK - 1) / kTK, (n + kTN - 1) / kTN);
+  int rc;
+  if ((rc = lora_attributes(smem)) != B200_OK) return rc;
   int C = 1;
-  while (C < 16 && expect * C * 2 <= 2 * lora_sms() && 2 * C <= steps) C *= 2;
+  int log_c = 0;
+  while (C < kMaxC && 2 * C <= steps && expect <= active_clusters(2 * C, smem)) {
+    C *= 2;
+    ++log_c;
+  }
   p.C = C;
+  p.log_c = log_c;
   if (tiles * C > 0x7fffffff) return B200_ERR_INVALID;
   CUtensorMap mx{}, ma{}, mb{}, my{};
-  int rc;
   if ((rc = lora_map(&mx, x, 2, k, rows, 1, ldx, 0, kTM)) != B200_OK) return rc;
   if ((rc = lora_map(&my, y, 2, n, rows, 1, ldy, 0, kTM)) != B200_OK) return rc;
   if (adapters > 0) {
     if ((rc = lora_map(&ma, a, 3, k, rank, adapters, k, static_cast<int64_t>(rank) * k, p.rp)) != B200_OK) return rc;
     if ((rc = lora_map(&mb, b, 3, rank, n, adapters, rank, static_cast<int64_t>(rank) * n, kTN)) != B200_OK) return rc;
-  }
-  if (cudaFuncSetAttribute(lora_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
-      cudaFuncSetAttribute(lora_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
-    cudaGetLastError();
-    return B200_ERR_CUDA;
   }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(tiles * C));
