@@ -18,7 +18,9 @@ time) and carries the end-to-end latents check.  Mirrors:
 Unlike the reference, which runs each sequence (prompt x {pos, neg}) as its own forward
 call, every sequence of a step goes through each block together: one GEMM per linear over
 all sequences' target tokens, one attention launch whose batch rows carry their own prefix
-lengths (b200_kv_desc) and RoPE tables (pe_batch_stride).  The residual stream is f32;
+lengths (b200_kv_desc) and RoPE tables (pe_batch_stride).  The prefix cache is dense bf16 or
+paged 4-bit (b200attn.kv4), and every sequence may carry a low-rank adapter of its own
+(b200attn.lora).  The residual stream is f32;
 GEMM operands are bf16 (cuBLAS through torch); attention, Q/K norm + RoPE and the
 elementwise block steps run in this package's CUDA library.
 """
@@ -257,6 +259,7 @@ class MMDiT:
                     qtype = bq.q4_k_m_type(name, i, cfg.layers)
                     blk["q_" + key] = bq.QuantLinear(bq.quantize(w.float(), qtype), qtype, tuple(w.shape))
                     del w
+        self.adapters = None
         self._bufs = {}
         # When a list, every attention call of the block loop appends its (start, end) CUDA
         # events (the attention kernel; with fused_qkv off, the b200_attn_fwd span of Q/K
@@ -397,11 +400,13 @@ class MMDiT:
 
     # -- the block loop -----------------------------------------------------------
     def _run_blocks(self, x, B: int, T: int, mod, pe, prefix: Optional[PrefixCache], desc,
-                    row_limit=None, kv_out: Optional[PrefixCache] = None, final_scale=None):
+                    row_limit=None, kv_out=None, final_scale=None, adapters=None):
         """x f32 [B*T, hidden] (updated in place) through every block; mod f32 [4*hidden]
-        (one row for every token).  Returns LN(x) * (1 + final_scale) bf16 when final_scale
-        is given (FinalLayer), else None."""
+        (one row for every token).  prefix and kv_out (the cache that this pass fills): a
+        PrefixCache or a KV4View.  adapters: adapter ids of the B sequences.  Returns LN(x) *
+        (1 + final_scale) bf16 when final_scale is given (FinalLayer), else None."""
         import torch
+        from b200attn.kv4 import KV4View
         cfg = self.cfg
         h, H, R = cfg.hidden, cfg.heads, B * T
         m = mod.view(1, 4 * h)
@@ -409,7 +414,12 @@ class MMDiT:
         y = self._buf("y", (R, h), torch.bfloat16)
         attn = self._buf("attn", (B, T, h), torch.bfloat16)
         ws_need = 2 * B * H * T * HEAD_DIM * 2 + b200attn.SPLIT_WORKSPACE_BYTES + 4096
+        paged = prefix if isinstance(prefix, KV4View) else None
+        if paged is not None:  # room to expand one layer's pages, beside the above
+            ws_need += b200attn.kv4_workspace_bytes(B, H, T, paged.max_len)
         ws = self._buf("ws", (ws_need,), torch.uint8)
+        lora = self._batch_adapters(adapters, B, T)
+        add_lora = (lambda *a: None) if lora is None else lora.add
         b200attn.residual_adaln(x, None, None, scale1, y, rows_per_mod=R)      # norm1 of block 0
         # A host-resident cache streams in one layer ahead: layer i's K/V land in staging
         # slot i % 2 on the copy stream while layer i - 1 computes; a slot is refilled only
@@ -437,8 +447,12 @@ class MMDiT:
         # A host-resident prefix pass (prefix_fill(offload=True)) writes each layer's K/V
         # into device staging slot i % 2 and drains it to the pinned host cache on the copy
         # stream while the next layer computes; a slot is rewritten only after its drain.
-        sink = None
-        if kv_out is not None and kv_out.on_host:
+        sink = quantised = None
+        if isinstance(kv_out, KV4View):  # each layer's K/V, before they go into its pages
+            shape = (B, H, T, HEAD_DIM)
+            quantised = (self._buf("kv4_k", shape, torch.bfloat16), self._buf("kv4_v", shape, torch.bfloat16))
+            counts = torch.tensor(kv_out.lengths, dtype=torch.int32, device=self.device)
+        elif kv_out is not None and kv_out.on_host:
             sink_stream = self._copy_stream()
             sink = self._staging("out", kv_out.k[0].shape)
             computed = [torch.cuda.Event() for _ in range(2)]
@@ -478,9 +492,12 @@ class MMDiT:
                     stage(i + 1)
                 cur.wait_event(landed[i % 2])
                 pk, pv = staged[i % 2]
-            elif prefix is not None:
+            elif prefix is not None and paged is None:
                 pk, pv = prefix.k[i], prefix.v[i]
-            fused = self.fused_qkv and kv_out is None and row_limit is None and H % 2 == 0
+            # (adapters change q and k before the norm: not with the fused epilogue)
+            fused = (self.fused_qkv and kv_out is None and row_limit is None and H % 2 == 0
+                     and lora is None)
+            name = f"transformer_blocks.{i}."
             if fused:   # projections + Q/K norm + RoPE in one GEMM, then the attention kernel
                 q_rot, k_rot, v = b200attn.qkv_norm_rope_gemm(
                     y, blk["wqkv"], B, T, H, blk["nq"], blk["nk"], pe,
@@ -491,24 +508,38 @@ class MMDiT:
                 q = self._gemm(y, blk["wq"], "q").view(B, T, H, HEAD_DIM)
                 k = self._gemm(y, blk["wk"], "k").view(B, T, H, HEAD_DIM)
                 v = self._gemm(y, blk["wv"], "v").view(B, T, H, HEAD_DIM)
+                add_lora(name + "attn.to_q", y, q.view(R, h))
+                add_lora(name + "attn.to_k", y, k.view(R, h))
+                add_lora(name + "attn.to_v", y, v.view(R, h))
             if self.attn_marks is not None:
                 ev = (torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True))
                 ev[0].record()
-            if fused:
+            if fused and paged is not None:
+                b200attn.kv4_joint_attention(q_rot, k_rot, v, paged.pool(i), paged.page_table,
+                                             paged.max_len, desc=desc, out=attn, workspace=ws)
+            elif fused:
                 b200attn.joint_attention(
                     q_rot, k_rot, v, pk, pv, desc=desc, out=attn,
                     workspace=ws[:b200attn.SPLIT_WORKSPACE_BYTES])
+            elif paged is not None:
+                b200attn.kv4_attention_forward(
+                    q, k, v, paged.pool(i), paged.page_table, paged.max_len, blk["nq"], blk["nk"], pe,
+                    desc=desc, out=attn, workspace=ws, row_limit=row_limit)
             else:
                 k_dst = v_dst = None
                 if sink is not None:
                     if drained[i % 2] is not None:
                         cur.wait_event(drained[i % 2])  # layer i - 2 has left this slot
                     k_dst, v_dst = sink[i % 2]
+                elif quantised is not None:
+                    k_dst, v_dst = quantised
                 elif kv_out is not None:
                     k_dst, v_dst = kv_out.k[i], kv_out.v[i]
                 b200attn.attention_forward(
                     q, k, v, pk, pv, blk["nq"], blk["nk"], pe, desc=desc,
                     out=attn, workspace=ws, row_limit=row_limit, k_rot_out=k_dst, v_out=v_dst)
+                if quantised is not None:
+                    kv_out.store(i, k_dst, v_dst, count=counts)
                 if sink is not None:
                     sl = i % 2
                     computed[sl].record(cur)
@@ -524,13 +555,17 @@ class MMDiT:
                 ev[1].record()
                 self.attn_marks.append(ev)
             o = self._gemm(attn.view(R, h), blk["wo"], "o")
+            add_lora(name + "attn.to_out.0", attn.view(R, h), o)
             b200attn.residual_adaln(x, o, gate1, scale2, y, rows_per_mod=R)    # attn residual, norm2
             mo = self._buf("mo", (R, h), torch.bfloat16)
             for r0 in range(0, R, self.mlp_chunk_rows):
                 r1 = min(R, r0 + self.mlp_chunk_rows)
                 gp = self._gemm(y[r0:r1], blk["wgp"], "gp")
+                add_lora(name + "img_mlp.gate_layer", y[r0:r1], gp[:, :cfg.ffn], r0)
+                add_lora(name + "img_mlp.proj", y[r0:r1], gp[:, cfg.ffn:], r0)
                 hh = b200attn.swiglu(gp, self._buf("h", (r1 - r0, cfg.ffn), torch.bfloat16))
                 self._gemm(hh, blk["wmo"], "mo", out=mo[r0:r1])
+                add_lora(name + "img_mlp.out", hh, mo[r0:r1], r0)
             last = i + 1 == len(self.blocks)
             if quant:
                 # (the residual kernel below reads no weights; the slot is free after mo)
@@ -549,6 +584,22 @@ class MMDiT:
                 b200attn.residual_adaln(x, mo, gate2, None, None, rows_per_mod=R)
         return None
 
+    # -- adapters --------------------------------------------------------------------
+    def set_adapters(self, bank) -> None:
+        """The adapter bank (b200attn.lora.AdapterBank) whose adapters prefix_fill, step and
+        denoise may name per sequence; None: none."""
+        self.adapters = bank
+
+    def _batch_adapters(self, ids, B: int, T: int):
+        if ids is None or all(i is None or i < 0 for i in ids):
+            return None
+        from b200attn.lora import BatchAdapters
+        if self.adapters is None:
+            raise ValueError("the model has no adapters (set_adapters)")
+        if len(ids) != B:
+            raise ValueError(f"{len(ids)} adapter ids for {B} sequences")
+        return BatchAdapters(self.adapters, ids, T)
+
     # -- prefix fill ---------------------------------------------------------------
     def text_embed(self, emb):
         """TextEmbedder::forward (src/transformer.rs:496-502): RMSNorm(w + 1) -> in_layer ->
@@ -560,7 +611,7 @@ class MMDiT:
         a = F.gelu((e.to(torch.bfloat16) @ self.txt_in1.t()).float(), approximate="tanh")
         return (a.to(torch.bfloat16) @ self.txt_in2.t()).float()
 
-    def prefix_fill(self, text_embs: Sequence, offload: bool = False) -> PrefixCache:
+    def prefix_fill(self, text_embs: Sequence, offload: bool = False, kv4=None, adapters=None):
         """prefix_kv (src/transformer.rs:674-707) for a batch of text-only prompts of ragged
         lengths, in one pass: the prompts are padded to Pmax rows, each row's descriptor
         limits its keys to its own length, and the text rows' causal mask
@@ -571,9 +622,15 @@ class MMDiT:
         layer's entry to the CPU as it is computed): the cache is allocated in pinned host
         memory up front and each layer's K/V goes through one of two reused device staging
         slots, drained to the host on a copy stream while the next layer computes, so the
-        device never holds more than two layers of it."""
+        device never holds more than two layers of it.
+
+        kv4 (a b200attn.kv4.KV4Cache): the prefixes become sequences of that cache, stored in
+        4 bits layer by layer; returns their KV4View instead of a PrefixCache.  adapters: the
+        adapter id of each prompt, or None."""
         import torch
         cfg = self.cfg
+        if kv4 is not None and offload:
+            raise ValueError("a 4-bit cache stays on the GPU")
         B = len(text_embs)
         lengths = [int(e.shape[0]) for e in text_embs]
         P = max(lengths)
@@ -582,19 +639,28 @@ class MMDiT:
             emb[b, :lengths[b]] = e.to(self.device, torch.bfloat16)
         x = self.text_embed(emb.view(B * P, cfg.text_dim)).contiguous()
         shape = (B, cfg.heads, P, HEAD_DIM)
-        if offload:
-            alloc = lambda: torch.empty(shape, dtype=torch.bfloat16).pin_memory()
+        if kv4 is not None:
+            cache = kv4.view(kv4.add(lengths))
         else:
-            alloc = lambda: torch.zeros(shape, dtype=torch.bfloat16, device=self.device)
-        cache = PrefixCache(k=[alloc() for _ in range(cfg.layers)],
-                            v=[alloc() for _ in range(cfg.layers)], lengths=lengths)
+            if offload:
+                alloc = lambda: torch.empty(shape, dtype=torch.bfloat16).pin_memory()
+            else:
+                alloc = lambda: torch.zeros(shape, dtype=torch.bfloat16, device=self.device)
+            cache = PrefixCache(k=[alloc() for _ in range(cfg.layers)],
+                                v=[alloc() for _ in range(cfg.layers)], lengths=lengths)
         lay = b200attn.joint_layout(P, None, [], (0, 0))
         pe = torch.from_numpy(b200attn.rope_pe(lay["img_shapes"], lay["image_pad_mask"], AXES,
                                                ROPE_THETA)[:P]).to(self.device)
         limits = torch.from_numpy(b200attn.block_causal_limits(lay["image_ids"][:P])).to(self.device)
         desc = torch.tensor([[0, n] for n in lengths], dtype=torch.int32, device=self.device)
         mod = self.modulation(self.zero_time_embed())
-        self._run_blocks(x, B, P, mod, pe, None, desc, row_limit=limits, kv_out=cache)
+        try:
+            self._run_blocks(x, B, P, mod, pe, None, desc, row_limit=limits, kv_out=cache,
+                             adapters=adapters)
+        except BaseException:
+            if kv4 is not None:
+                kv4.free(cache.seqs)
+            raise
         return cache
 
     def target_pe(self, lengths: Sequence[int], grid: Tuple[int, int]):
@@ -609,9 +675,10 @@ class MMDiT:
         return torch.from_numpy(np.stack(rows)).to(self.device).contiguous()
 
     # -- one cached step --------------------------------------------------------------
-    def step(self, lat, t: float, cache: PrefixCache, pe, desc):
+    def step(self, lat, t: float, cache, pe, desc, adapters=None):
         """The cached forward_conditioned of every sequence at timestep t: lat [B, T, C]
-        (bf16 or f32) -> velocity f32 [B, T, C]."""
+        (bf16 or f32) -> velocity f32 [B, T, C].  cache: a PrefixCache or a KV4View; adapters:
+        the adapter id of each sequence, or None."""
         import torch
         cfg = self.cfg
         B, T, C = lat.shape
@@ -620,13 +687,13 @@ class MMDiT:
         x.copy_(x_in)
         t_emb = self.time_embed(t)
         y = self._run_blocks(x, B, T, self.modulation(t_emb), pe, cache, desc,
-                             final_scale=self.final_scale(t_emb))
+                             final_scale=self.final_scale(t_emb), adapters=adapters)
         out = self._buf("pred", (B * T, C), torch.bfloat16)
         torch.mm(y, self.proj_out.t(), out=out)
         return out.view(B, T, C).float()
 
 
-def cached_desc(cache: PrefixCache, target_len: int, device):
+def cached_desc(cache, target_len: int, device):
     """Key descriptors of a cached step: each sequence sees its own prefix and every target
     key (src/transformer.rs:642-649 with key_valid None)."""
     import torch
@@ -634,30 +701,57 @@ def cached_desc(cache: PrefixCache, target_len: int, device):
 
 
 def denoise(model: MMDiT, pos_embs: Sequence, neg_embs: Optional[Sequence], grid: Tuple[int, int],
-            steps: int, cfg_scale: float, noise, step_callback=None, offload_cache: bool = False):
+            steps: int, cfg_scale: float, noise, step_callback=None, offload_cache: bool = False,
+            kv4=None, adapters=None):
     """denoise (src/pipeline.rs:126-197) for a batch of prompts: noise f32 [n_prompts, T, C]
     (packed), one prefix cache for every positive and negative prompt, `steps` Euler steps
     with true CFG (neg + scale * (pos - neg)) when neg_embs is given.  Latents stay f32;
     the transformer reads them as bf16.  offload_cache keeps the prefix cache in pinned host
-    memory (set_kv_cache_offload).  Returns the final packed latents f32 [n, T, C]."""
+    memory (set_kv_cache_offload).  kv4 (a b200attn.kv4.KV4Cache, True: one made to fit)
+    keeps it in 4 bits; prompts that are given as one and the same tensor, like a negative
+    prompt for every request, are then computed once and share their pages, which are free
+    again at the end.  adapters: the adapter id of each prompt (its negative takes the same),
+    or None.  Returns the final packed latents f32 [n, T, C]."""
     import torch
     n = noise.shape[0]
     T = grid[0] * grid[1]
     embs = list(pos_embs)
     if neg_embs is not None:  # sequence order: p0 pos, p0 neg, p1 pos, p1 neg, ...
         embs = [e for pair in zip(pos_embs, neg_embs) for e in pair]
-    cache = model.prefix_fill(embs, offload=offload_cache)
-    pe = model.target_pe(cache.lengths, grid)
-    desc = cached_desc(cache, T, model.device)
-    sigmas = flow_match_sigmas(steps, T)
-    lat = noise.to(model.device, torch.float32).clone()
-    for i in range(steps):
-        x_in = lat.repeat_interleave(2, 0) if neg_embs is not None else lat
-        pred = model.step(x_in, float(sigmas[i]), cache, pe, desc)
-        if neg_embs is not None:
-            pos, neg = pred[0::2], pred[1::2]
-            pred = neg + (pos - neg) * cfg_scale
-        lat = lat + pred * euler_dt(sigmas, i)
-        if step_callback is not None:
-            step_callback(i)
-    return lat
+    ids = adapters
+    if adapters is not None and neg_embs is not None:
+        ids = [a for a in adapters for _ in range(2)]
+    seqs: List[int] = []
+    if kv4 is not None and kv4 is not False:
+        from b200attn.kv4 import KV4Cache
+        keys = [(id(e), None if ids is None else ids[i]) for i, e in enumerate(embs)]
+        first = [keys.index(k) for k in keys]
+        once = sorted(set(first))
+        if kv4 is True:
+            kv4 = KV4Cache(model.cfg.layers, model.cfg.heads,
+                           KV4Cache.pages_for([int(embs[i].shape[0]) for i in once]), model.device)
+        filled = model.prefix_fill([embs[i] for i in once], kv4=kv4,
+                                   adapters=None if ids is None else [ids[i] for i in once])
+        own = dict(zip(once, filled.seqs))
+        seqs = [own[i] if i == f else kv4.fork([own[f]])[0] for i, f in enumerate(first)]
+        cache = kv4.view(seqs)
+    else:
+        cache = model.prefix_fill(embs, offload=offload_cache, adapters=ids)
+    try:
+        pe = model.target_pe(cache.lengths, grid)
+        desc = cached_desc(cache, T, model.device)
+        sigmas = flow_match_sigmas(steps, T)
+        lat = noise.to(model.device, torch.float32).clone()
+        for i in range(steps):
+            x_in = lat.repeat_interleave(2, 0) if neg_embs is not None else lat
+            pred = model.step(x_in, float(sigmas[i]), cache, pe, desc, adapters=ids)
+            if neg_embs is not None:
+                pos, neg = pred[0::2], pred[1::2]
+                pred = neg + (pos - neg) * cfg_scale
+            lat = lat + pred * euler_dt(sigmas, i)
+            if step_callback is not None:
+                step_callback(i)
+        return lat
+    finally:
+        if seqs:
+            kv4.free(seqs)

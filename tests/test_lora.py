@@ -10,6 +10,9 @@ import pytest
 import torch
 
 import b200attn
+from b200attn import mmdit
+from b200attn.lora import TARGETS, AdapterBank, BatchAdapters
+from oracle import mmdit_ref as M
 
 
 def lib_call(rows=4, segments=2, adapters=3, n=64, k=64, rank=16, ldx=None, ldy=None, ldo=None, x=16, y=16,
@@ -157,3 +160,105 @@ def test_bad_adapters_and_segments_stay_in_bounds(cuda):
                             out=torch.zeros(50, 64, dtype=torch.bfloat16, device=cuda), status=status)
     assert status.item() == b200attn.LORA_STATUS_BAD_ADAPTER
     check(got, x, y, a, b, scale, torch.tensor([0, 10, 30, 50]), torch.tensor([0, -1, 1]))
+
+
+@pytest.mark.gpu
+def test_captured_and_on_another_stream(cuda):
+    """A captured call replayed with other adapters, rows and inputs, and a call on a stream
+    of its own, equal the plain call."""
+    g = torch.Generator().manual_seed(8)
+    x, y, a, b, scale, seg, who = (t.to(cuda) for t in make(g, [70, 130, 1], [0, 1, -1], 512, 384, 16, 2))
+    out = torch.empty_like(y)
+    call = lambda stream=None: b200attn.lora_add(x, a, b, y, seg, who, scale=scale, out=out, stream=stream)
+    plain = call().clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    out.zero_()
+    torch.cuda.synchronize()
+    call(side)
+    side.synchronize()
+    assert torch.equal(out, plain)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    x.copy_(torch.randn(x.shape, generator=g))
+    seg.copy_(torch.tensor([0, 1, 200, 201]))
+    who.copy_(torch.tensor([1, -1, 0]))
+    graph.replay()
+    replayed = out.clone()
+    out.zero_()
+    assert torch.equal(replayed, call()) and not torch.equal(replayed, plain)
+
+
+# ----------------------------------------------------------------- the model's adapters
+TINY = mmdit.MMDiTConfig(layers=2, heads=2, text_dim=256)
+GRID = (16, 16)
+
+
+def _adapter(g, rank, names):
+    shapes = {k[:-len(".weight")]: v for k, v in mmdit.weight_shapes(TINY).items()}
+    return {n: (torch.randn(rank, shapes[n][1], generator=g) * shapes[n][1] ** -0.5,
+                torch.randn(shapes[n][0], rank, generator=g) * 0.1) for n in names}
+
+
+def _names(layer, targets=TARGETS):
+    return [f"transformer_blocks.{layer}.{t}" for t in targets]
+
+
+def test_bank_refuses_what_does_not_fit():
+    g = torch.Generator().manual_seed(0)
+    good = _adapter(g, 4, _names(0))
+    bank = AdapterBank([good], device="cpu")
+    assert bank.linears["transformer_blocks.0.attn.to_q"][0].shape == (1, 8, 256)  # ranks in eights
+    with pytest.raises(ValueError):
+        AdapterBank([], device="cpu")
+    with pytest.raises(ValueError, match="scale"):
+        AdapterBank([good], scales=[1.0, 2.0], device="cpu")
+    with pytest.raises(ValueError, match="block linear"):
+        AdapterBank([{"proj_out": (torch.zeros(4, 8), torch.zeros(8, 4))}], device="cpu")
+    n = "transformer_blocks.0.attn.to_q"
+    with pytest.raises(ValueError, match="fit together"):
+        AdapterBank([{n: (torch.zeros(4, 8), torch.zeros(8, 5))}], device="cpu")
+    with pytest.raises(ValueError, match="fit together"):
+        AdapterBank([{n: (torch.zeros(4, 8), torch.zeros(8, 4))}, {n: (torch.zeros(4, 16), torch.zeros(8, 4))}],
+                    device="cpu")
+    with pytest.raises(ValueError, match="rank"):
+        AdapterBank([{n: (torch.zeros(130, 8), torch.zeros(8, 130))}], device="cpu")
+    with pytest.raises(ValueError, match="adapters"):
+        BatchAdapters(bank, [1], 4)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["bf16", "q4_k_m"])
+def test_every_sequence_with_its_own_adapter(cuda, fmt):
+    """A batched prefix fill and step whose sequences carry different adapters (of different
+    ranks, on different linears, or none) against the float32 oracle with each adapter merged
+    into the weights, sequence by sequence; the MLP in chunks that cut sequences."""
+    w = mmdit.random_weights(TINY, 0, std=0.1)
+    model = mmdit.MMDiT(TINY, w, device=cuda, weight_format=fmt, mlp_chunk_rows=200)
+    g = torch.Generator().manual_seed(11)
+    adapters = [_adapter(g, 8, _names(0) + _names(1)), _adapter(g, 20, _names(1, TARGETS[2:5]))]
+    scales = [0.7, 1.3]
+    model.set_adapters(AdapterBank(adapters, scales, cuda))
+    lengths, ids = [40, 72, 65], [1, None, 0]
+    embs = [torch.randn(n, 256, generator=g).to(torch.bfloat16) for n in lengths]
+    lat = torch.randn(3, 256, 64, generator=g)
+    cache = model.prefix_fill(embs, adapters=ids)
+    got = model.step(lat.to(cuda), 0.5, cache, model.target_pe(lengths, GRID),
+                     mmdit.cached_desc(cache, 256, cuda), adapters=ids).cpu()
+    base = model.effective_weights(w)
+    for b, e in enumerate(ids):
+        merged = dict(base)
+        if e is not None:
+            for name, (A, B) in adapters[e].items():
+                merged[name + ".weight"] = base[name + ".weight"].float() + scales[e] * (
+                    B.bfloat16().float() @ A.bfloat16().float())
+        R = M.Reference(merged, TINY.layers, TINY.heads)
+        want = R.forward_cached(lat[b], 0.5, R.prefix_kv(embs[b].float(), GRID), lengths[b], GRID)
+        rel = float((got[b].double() - want.double()).norm() / want.double().norm())
+        assert rel <= 1.5e-2, (b, rel)
+    with pytest.raises(ValueError, match="adapter ids"):
+        model.prefix_fill(embs, adapters=[0])
+    model.set_adapters(None)
+    with pytest.raises(ValueError, match="no adapters"):
+        model.prefix_fill(embs, adapters=ids)
