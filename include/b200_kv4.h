@@ -84,7 +84,8 @@ int b200_kv4_load(const b200_kv4_view* cache, const int32_t* lengths, int32_t le
                   void* k_out, void* v_out, int32_t batch, int32_t heads, int32_t max_len,
                   int32_t head_dim, int32_t* status, b200_stream_t stream);
 
-/* Scratch bytes of b200_kv4_joint_attention for these sizes (0 where it needs none). */
+/* Scratch bytes of b200_kv4_joint_attention for these sizes; 0 for few query rows (up to 64,
+ * and up to 128 where batch * heads <= 64). */
 int b200_kv4_attention_workspace_bytes(int32_t batch, int32_t heads, int32_t target_len,
                                        int32_t prefix_len, size_t* bytes);
 
@@ -99,12 +100,11 @@ int b200_kv4_attention_workspace_bytes(int32_t batch, int32_t heads, int32_t tar
  * reach the output, infinities and NaN included.  A row without any key gives NaN (the
  * reference's softmax of a row of -inf).
  *
- * Few query rows run as one kernel straight from the 4-bit pages; from
- * B200_KV4_DENSE_QUERIES rows on, the pages are expanded into the workspace once
- * (b200_kv4_load's kernel) and the tensor-core attention kernel reads them there.  Both
- * work on the same values.  Calls that may overlap need workspaces of their own.
+ * Few query rows run as one kernel straight from the 4-bit pages, without a workspace; for
+ * more, the pages are expanded into the workspace once (b200_kv4_load's kernel) and the
+ * tensor-core attention kernel reads them there.  Both work on the same values.  Calls that
+ * may overlap need workspaces of their own.
  */
-#define B200_KV4_DENSE_QUERIES 65
 int b200_kv4_joint_attention(const b200_kv4_view* cache, const void* q_rot, const void* k_rot,
                              const void* v, int32_t batch, int32_t heads, int32_t target_len,
                              int32_t prefix_len, int32_t head_dim, const b200_kv_desc* desc,

@@ -573,7 +573,6 @@ def qkv_norm_rope_gemm(x, w_qkv, batch: int, tokens: int, heads: int, norm_q_w, 
 
 # ----------------------------------------------------------------- paged 4-bit prefix cache
 KV4_PAGE_TOKENS, KV4_BLOCK_BYTES = 64, 9216
-KV4_DENSE_QUERIES = 65   # B200_KV4_DENSE_QUERIES
 KV4_STATUS_BAD_PAGE = 16
 
 
@@ -684,8 +683,7 @@ def kv4_joint_attention(q_rot, k_rot, v, pool, page_table, prefix_len: int, desc
     v bf16 [B,T,H,D], pool uint8 [num_pages, H, 9216], page_table int32 [B, max_pages] -> out
     bf16 [B,T,H*D].  prefix_len bounds every desc[b].prefix_valid (desc int32 [B, 2] or None:
     prefix_len and T).  row_limit int32 [T] or None: row i sees this call's keys
-    [0, row_limit[i]).  workspace uint8 (kv4_workspace_bytes; needed from
-    KV4_DENSE_QUERIES tokens on, allocated here when None)."""
+    [0, row_limit[i]).  workspace uint8 (kv4_workspace_bytes; allocated here when None)."""
     import torch
     b, h, t, d = q_rot.shape
     dev = pool.device
@@ -703,9 +701,9 @@ def kv4_joint_attention(q_rot, k_rot, v, pool, page_table, prefix_len: int, desc
             out = q_rot.new_empty((b, t, h * d))
         else:
             _expect(out, "out", bf, (b, t, h * d), dev)
-        if workspace is None and t >= KV4_DENSE_QUERIES:
-            workspace = torch.empty(kv4_workspace_bytes(b, h, t, prefix_len), dtype=torch.uint8,
-                                    device=dev)
+        if workspace is None and t > 64:  # up to there it needs none
+            workspace = torch.empty(max(1, kv4_workspace_bytes(b, h, t, prefix_len)),
+                                    dtype=torch.uint8, device=dev)
         ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
         _check(lib().b200_kv4_joint_attention(
             ctypes.byref(view), _dptr(q_rot), _dptr(k_rot), _dptr(v), b, h, t, int(prefix_len), d,

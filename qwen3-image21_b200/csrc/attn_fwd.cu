@@ -1172,6 +1172,12 @@ int joint_attention(const void* q_rot, const void* k_rot, const void* v, const v
                           counters_zeroed);
 }
 
+int32_t* split_counters(void* split_region, int* n) {
+  *n = kMaxSplitSlots;
+  return reinterpret_cast<int32_t*>(static_cast<uint8_t*>(split_region) +
+                                    size_t{kMaxSplitSlots} * kSplitSlotBytes);
+}
+
 int attn_prologue(const b200_attn_args& a, void* q_rot, void* k_rot, cudaStream_t stream) {
   NormRopeJob jobs[3] = {
       {static_cast<const __nv_bfloat16*>(a.q), static_cast<__nv_bfloat16*>(q_rot), a.norm_q_w},

@@ -20,6 +20,10 @@ int joint_attention(const void* q_rot, const void* k_rot, const void* v, const v
                     cudaStream_t stream, bool counters_zeroed = false,
                     const int32_t* row_limit = nullptr);
 
+// The arrival counters of a split region, which are zero before the launch: `n` words that
+// the caller clears where it says counters_zeroed.
+int32_t* split_counters(void* split_region, int* n);
+
 // Q/K RMSNorm + RoPE of args (and the copy of V to v_out, if given) into q_rot and k_rot.
 int attn_prologue(const b200_attn_args& args, void* q_rot, void* k_rot, cudaStream_t stream);
 

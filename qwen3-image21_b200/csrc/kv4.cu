@@ -88,7 +88,8 @@ __device__ __forceinline__ uint32_t less_of(uint32_t step2) {  // -24 s, exact
 __device__ __forceinline__ float group_step(float top) {
   if (!(top < kHuge)) return __uint_as_float(0x7fc00000u);  // infinity, NaN, or too large
   if (top < kTiny) return 0.f;
-  return __uint_as_float(__float_as_uint(top * (0.14285714285714285 * (1.0 + 0x1p-20))) & 0xfff80000u);
+  constexpr float kSeventh = static_cast<float>(1.0 / 7.0 * (1.0 + 0x1p-20));
+  return __uint_as_float(__float_as_uint(top * kSeventh) & 0xfff80000u);
 }
 
 // The factor that number4 takes for a step (0 for a step of 0 or NaN, whose numbers are 0).
@@ -137,7 +138,7 @@ struct StoreParams {
 // 2t + {0, 1}, channels 32c + 4g + i — what the block wants of it as one 16-byte word per
 // octet — so nothing is exchanged but the group maxima (over t for K, over g for V).  Global
 // reads are 64-byte runs, stores 512-byte runs.
-__global__ void __launch_bounds__(128) kv4_store_kernel(const StoreParams p) {
+__global__ void __launch_bounds__(128, 6) kv4_store_kernel(const StoreParams p) {
   const int b = blockIdx.z, h = blockIdx.y;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t = lane & 3;
@@ -147,13 +148,8 @@ __global__ void __launch_bounds__(128) kv4_store_kernel(const StoreParams p) {
   const int64_t page_i = (first >= 0 ? first / kPage : -((-first + kPage - 1) / kPage)) + blockIdx.x;
   const int64_t base = page_i * kPage + warp * 16;  // position of this warp's first token
   if (base + 16 <= first || base >= first + n) return;
-  int page = -1;
+  int page = -1;  // looked at after the loads of k and v are on their way
   if (page_i >= 0 && page_i < p.max_pages) page = p.table[static_cast<int64_t>(b) * p.max_pages + page_i];
-  if (page < 0 || page >= p.num_pages) {
-    if (lane == 0) report_bad_page(p.status);
-    return;
-  }
-  uint8_t* block = p.pool + (static_cast<int64_t>(page) * p.heads + h) * kBlock;
   const __nv_bfloat16* kb = p.k + b * p.k_sb + h * p.k_sh;
   const __nv_bfloat16* vb = p.v + b * p.v_sb + h * p.v_sh;
   const int64_t i0 = base - first;  // index of the warp's first token in k and v
@@ -177,6 +173,11 @@ __global__ void __launch_bounds__(128) kv4_store_kernel(const StoreParams p) {
                                : make_uint2(0, 0);
     }
   }
+  if (page < 0 || page >= p.num_pages) {
+    if (lane == 0) report_bad_page(p.status);
+    return;
+  }
+  uint8_t* block = p.pool + (static_cast<int64_t>(page) * p.heads + h) * kBlock;
 #pragma unroll
   for (int o = 0; o < 2; ++o) {
     const int octet = 2 * warp + o;
@@ -251,10 +252,14 @@ struct LoadParams {
   __nv_bfloat16 *k, *v;    // [B][H][max_len][128]
   int32_t heads, max_len;
   int32_t* status;
+  int32_t* zero;  // n_zero words to clear for the launch behind this one, or NULL
+  int32_t n_zero;
 };
 
 // grid (page, head, batch row), lanes as in the store.
 __global__ void __launch_bounds__(128) kv4_load_kernel(const LoadParams p) {
+  if (p.zero && blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0)
+    for (int i = threadIdx.x; i < p.n_zero; i += 128) p.zero[i] = 0;
   const int b = blockIdx.z, h = blockIdx.y;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t = lane & 3;
@@ -907,10 +912,11 @@ constexpr int kMaxLen = 0x7fff0000;  // positions, rounded up to pages, stay in 
 
 // Launches kv4_load_kernel; arguments are validated.
 int launch_load(const b200_kv4_view& c, const int32_t* lengths, int length_stride, void* k, void* v,
-                int batch, int heads, int max_len, int32_t* status, cudaStream_t stream) {
+                int batch, int heads, int max_len, int32_t* status, cudaStream_t stream,
+                int32_t* zero = nullptr, int n_zero = 0) {
   LoadParams p{static_cast<const uint8_t*>(c.pool), c.page_table, c.num_pages, c.max_pages, lengths,
                length_stride, static_cast<__nv_bfloat16*>(k), static_cast<__nv_bfloat16*>(v), heads,
-               max_len, status};
+               max_len, status, zero, n_zero};
   const dim3 grid((max_len + kPage - 1) / kPage, heads, batch);
   kv4_load_kernel<<<grid, 128, 0, stream>>>(p);
   return cudaGetLastError() == cudaSuccess ? B200_OK : B200_ERR_CUDA;
@@ -987,6 +993,17 @@ int launch_few_rows(const b200_kv4_view& c, const void* q, const void* k, const 
 }
 
 size_t round256(size_t x) { return (x + 255) / 256 * 256; }
+
+// Whether the pages are read by the few-row kernel or expanded for the tensor-core kernel.
+// Per page, head and 16 rows the former takes 0.38 us of an SM; the latter takes the
+// expansion's 0.6 KB per token and head at HBM rate, and its 256-row tiles cost the same for
+// 1 row.  64 against 65 rows: 992 and 1205 us for 16 x 32 heads over 10.6k tokens, 140 and
+// 149 us for 4 x 32 over 5k; 80 rows: 1232 and 1202 us, 176 and 151 us.  With few heads in
+// all the dense tiles leave SMs idle, and the pages win up to 128 rows: 32 heads, 128 rows,
+// 17.4 and 17.8 us over 512 tokens, 148 and 192 us over 10.6k; 160 rows: 21.6 and 20.1 us.
+bool few_rows(int64_t batch, int64_t heads, int target_len) {
+  return target_len <= 64 || (target_len <= 128 && batch * heads <= 64);
+}
 
 size_t dense_bytes(int batch, int heads, int prefix_len) {
   return round256(static_cast<size_t>(batch) * heads * prefix_len * kHeadDim * 2);
@@ -1081,7 +1098,7 @@ extern "C" int b200_kv4_copy_pages(void* pool, int32_t layers, int64_t layer_str
 extern "C" int b200_kv4_attention_workspace_bytes(int32_t batch, int32_t heads, int32_t target_len,
                                                   int32_t prefix_len, size_t* bytes) {
   if (!bytes || batch < 0 || heads < 0 || target_len < 0 || prefix_len < 0) return B200_ERR_INVALID;
-  *bytes = target_len < B200_KV4_DENSE_QUERIES
+  *bytes = few_rows(batch, heads, target_len)
                ? 0
                : 2 * dense_bytes(batch, heads, prefix_len) + B200_ATTN_SPLIT_WORKSPACE_BYTES;
   return B200_OK;
@@ -1107,7 +1124,7 @@ extern "C" int b200_kv4_joint_attention(const b200_kv4_view* c, const void* q_ro
     if (!al16(ptr)) return B200_ERR_INVALID;
   if (!(scale > 0.f) || !std::isfinite(scale)) return B200_ERR_INVALID;
   auto stream = static_cast<cudaStream_t>(stream_);
-  if (target_len < B200_KV4_DENSE_QUERIES)
+  if (few_rows(batch, heads, target_len))
     return launch_few_rows(*c, q_rot, k_rot, v, batch, heads, target_len, prefix_len, desc, row_limit,
                            scale, out, status, stream);
   size_t need = 0;
@@ -1115,13 +1132,15 @@ extern "C" int b200_kv4_joint_attention(const b200_kv4_view* c, const void* q_ro
   if (need > 0 && (!workspace || workspace_bytes < need)) return B200_ERR_WORKSPACE;
   auto* ws = static_cast<uint8_t*>(workspace);
   const size_t one = dense_bytes(batch, heads, prefix_len);
+  int n_zero = 0;
+  int32_t* counters = split_counters(ws + 2 * one, &n_zero);
   if (prefix_len > 0) {
     rc = launch_load(*c, desc ? &desc[0].prefix_valid : nullptr, 2, ws, ws + one, batch, heads,
-                     prefix_len, status, stream);
+                     prefix_len, status, stream, counters, n_zero);
     if (rc != B200_OK) return rc;
   }
   return joint_attention(q_rot, k_rot, v, ws, ws + one, batch, heads, target_len, prefix_len, desc,
-                         scale, out, status, ws + 2 * one, stream, false, row_limit);
+                         scale, out, status, ws + 2 * one, stream, prefix_len > 0, row_limit);
 }
 
 extern "C" int b200_kv4_attn_workspace_bytes(const b200_attn_args* a, size_t* bytes) {

@@ -184,7 +184,7 @@ def test_fork_extend_free_compact_and_attend(cuda):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("tokens", [4, 80])
+@pytest.mark.parametrize("tokens", [4, 150])
 def test_captured_and_on_another_stream(cuda, tokens):
     """A captured store and attention replayed on new inputs and a new page table, and the
     same calls on a stream of their own, equal the plain calls."""
@@ -296,7 +296,7 @@ def test_denoise_shares_the_negative_prompt(cuda):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("tokens", [3, 96])
+@pytest.mark.parametrize("tokens", [3, 150])
 def test_attention_forward_is_norm_rope_and_attention(cuda, tokens):
     g = torch.Generator().manual_seed(tokens)
     heads, n, b = 4, 90, 2
