@@ -765,16 +765,18 @@ def kv4_copy_pages(pool, src: Sequence[int], dst: Sequence[int], stream=None):
     9216] (or one layer's [num_pages, H, 9216]).  src and dst are host sequences; a page that
     is written twice, or both read and written, is refused (B200Error ERR_INVALID)."""
     import torch
-    if pool.dim() == 3:
-        pool = pool.unsqueeze(0)
-    _expect(pool, "pool", torch.uint8, (*pool.shape[:3], KV4_BLOCK_BYTES), pool.device)
-    if len(src) != len(dst):
-        raise ValueError("src and dst must have the same length")
+    if pool.dim() not in (3, 4):
+        raise ValueError("pool must have 3 or 4 dimensions")
+    pages, heads = pool.shape[-3:-1]
+    layers = pool.shape[0] if pool.dim() == 4 else 1
+    _expect(pool, "pool", torch.uint8, (*pool.shape[:-1], KV4_BLOCK_BYTES), pool.device)
     n = len(src)
+    if n != len(dst):
+        raise ValueError("src and dst must have the same length")
     s, d = (ctypes.c_int32 * n)(*src), (ctypes.c_int32 * n)(*dst)
     with _Launch(pool, stream) as st:
-        _check(lib().b200_kv4_copy_pages(_dptr(pool), pool.shape[0], pool.stride(0), pool.shape[1],
-                                         pool.shape[2], s, d, n, st), "b200_kv4_copy_pages")
+        _check(lib().b200_kv4_copy_pages(_dptr(pool), layers, pages * heads * KV4_BLOCK_BYTES, pages,
+                                         heads, s, d, n, st), "b200_kv4_copy_pages")
 
 
 # ----------------------------------------------------------------- per-request adapters

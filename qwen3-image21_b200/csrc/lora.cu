@@ -38,9 +38,10 @@ constexpr int kXBytes = kTM * kTK * 2;   // x tile, or y tile: 16 KiB
 constexpr int kLThreads = 256;
 constexpr uint32_t kLTmemCols = 256;     // u: 128 columns, two accumulators of 64
 constexpr uint32_t kAccCol = 128;
-constexpr int kMaxStages = 4;
+constexpr int kMaxStages = 8;
 constexpr int kMaxC = 16;
 constexpr int kMaxExtent = 1 << 30;      // of K and N
+constexpr int kBarBytes = 512;
 // Columns times groups of 4 rows of u up to which every CTA of a cluster adds the partials up
 // for itself, which saves one exchange between the CTAs.
 constexpr int kDirect = 256;
@@ -135,14 +136,15 @@ __device__ __forceinline__ uint32_t lora_pack(float lo, float hi) {
 
 __device__ __forceinline__ void epi_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
-// The request and rows of tile `tile`; all lanes of one warp call it.  Returns the number of
+// The adapter and rows of tile `tile`; all lanes of one warp call it.  Returns the number of
 // rows, 0 when there is no such tile.
-__device__ __forceinline__ int find_tile(const LoraParams& p, int tile, int lane, int& seg, int& row0) {
+__device__ __forceinline__ int find_tile(const LoraParams& p, int tile, int lane, int& adapter, int& row0) {
   int before = 0;
   for (int s0 = 0; s0 < p.segments; s0 += 32) {
     const int s = s0 + lane;
-    int lo = 0, len = 0;
+    int lo = 0, len = 0, mine_adapter = -1;
     if (s < p.segments) {
+      mine_adapter = p.seg_adapter[s];
       lo = min(max(p.seg_start[s], 0), p.rows);
       len = max(min(p.seg_start[s + 1], p.rows) - lo, 0);
     }
@@ -159,7 +161,7 @@ __device__ __forceinline__ int find_tile(const LoraParams& p, int tile, int lane
       const int who = __ffs(hit) - 1;
       const int skip = tile - before - (__shfl_sync(0xffffffffu, sum - mine, who));
       const int base = __shfl_sync(0xffffffffu, lo, who), rows = __shfl_sync(0xffffffffu, len, who);
-      seg = s0 + who;
+      adapter = __shfl_sync(0xffffffffu, mine_adapter, who);
       row0 = base + skip * kTM;
       return min(kTM, rows - skip * kTM);
     }
@@ -206,7 +208,7 @@ __global__ void __launch_bounds__(kLThreads, 2)
   uint64_t* part_ready = u_full + 6;          // every CTA's partials are written
   uint64_t* slice_ready = u_full + 7;         // every CTA's rows are reduced (and partials read)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(u_full + 8);
-  int* tile_word = reinterpret_cast<int*>(u_full + 9);  // [3]: rows, segment, first row
+  int* tile_word = reinterpret_cast<int*>(u_full + 9);  // [3]: rows, adapter, first row
   volatile int* abort_flag = tile_word + 3;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -237,12 +239,12 @@ __global__ void __launch_bounds__(kLThreads, 2)
     tmem_relinquish();
   }
   if (warp == 3) {
-    int seg = 0, row0 = 0;
-    const int rows = find_tile(p, blockIdx.x / C, lane, seg, row0);
+    int of = -1, first = 0;
+    const int n = find_tile(p, blockIdx.x / C, lane, of, first);
     if (lane == 0) {
-      tile_word[0] = rows;
-      tile_word[1] = seg;
-      tile_word[2] = row0;
+      tile_word[0] = n;
+      tile_word[1] = of;
+      tile_word[2] = first;
     }
   }
   tc_fence_before();
@@ -250,7 +252,7 @@ __global__ void __launch_bounds__(kLThreads, 2)
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   const int rows = tile_word[0], row0 = tile_word[2];
-  int adapter = rows > 0 ? p.seg_adapter[tile_word[1]] : -1;
+  int adapter = rows > 0 ? tile_word[1] : -1;
   if (adapter >= p.adapters) {
     if (threadIdx.x == 0 && p.status) atomicCAS(p.status, 0, B200_LORA_STATUS_BAD_ADAPTER);
     adapter = -1;
@@ -668,9 +670,8 @@ extern "C" int b200_lora_add(const void* x, int64_t ldx, const void* a, const vo
   p.rp = (rank + 15) / 16 * 16;
   p.status = status;
   const int regions = p.rp > 64 ? 2 : 1;
-  p.stages = 3 + (regions - 1);
   p.stage_bytes = kXBytes + regions * kTN * kTK * 2;
-  const int smem = p.stages * p.stage_bytes + regions * kXBytes + 256 + 1024;
+  const auto smem_of = [&](int stages) { return stages * p.stage_bytes + regions * kXBytes + kBarBytes + 1024; };
   // Every request ends in a tile of its own: rows / 128 + segments tiles at most.  The
   // cluster is the largest whose tiles are expected to run all at once: with every request's
   // last tile half full on average.
@@ -678,15 +679,18 @@ extern "C" int b200_lora_add(const void* x, int64_t ldx, const void* a, const vo
   const int64_t expect = std::min<int64_t>(tiles, (rows + kTM - 1) / kTM + segments / 2);
   const int steps = std::max((k + kTK - 1) / kTK, (n + kTN - 1) / kTN);
   int rc;
-  if ((rc = lora_attributes(smem)) != B200_OK) return rc;
-  int C = 1;
-  int log_c = 0;
-  while (C < kMaxC && 2 * C <= steps && expect <= active_clusters(2 * C, smem)) {
-    C *= 2;
-    ++log_c;
+  if ((rc = lora_attributes(smem_of(regions == 1 ? 7 : 6))) != B200_OK) return rc;
+  // The ring: 3 stages with two CTAs per SM, or (rank over 64) 4 with one; where one CTA per
+  // SM holds all tiles in clusters as large, the rest of its shared memory too.
+  p.stages = regions == 1 ? 3 : 4;
+  p.C = 1;
+  while (p.C < kMaxC && 2 * p.C <= steps && expect <= active_clusters(2 * p.C, smem_of(p.stages))) {
+    p.C *= 2;
+    ++p.log_c;
   }
-  p.C = C;
-  p.log_c = log_c;
+  const int deep = regions == 1 ? 7 : 6;
+  if (expect <= active_clusters(p.C, smem_of(deep))) p.stages = deep;
+  const int C = p.C, smem = smem_of(p.stages);
   if (tiles * C > 0x7fffffff) return B200_ERR_INVALID;
   CUtensorMap mx{}, ma{}, mb{}, my{};
   if ((rc = lora_map(&mx, x, 2, k, rows, 1, ldx, 0, kTM)) != B200_OK) return rc;
