@@ -85,7 +85,7 @@ int b200_kv4_load(const b200_kv4_view* cache, const int32_t* lengths, int32_t le
                   int32_t head_dim, int32_t* status, b200_stream_t stream);
 
 /* Scratch bytes of b200_kv4_joint_attention for these sizes; 0 for few query rows (up to 64,
- * and up to 128 where batch * heads <= 64). */
+ * and up to 128 where batch * heads <= 64 and prefix_len >= 4 * target_len). */
 int b200_kv4_attention_workspace_bytes(int32_t batch, int32_t heads, int32_t target_len,
                                        int32_t prefix_len, size_t* bytes);
 

@@ -475,6 +475,19 @@ template <int J>
 struct WarpState {
   float m[J][2], less[J][2], l[J][2];
   float o[8][J][4];
+
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      m[j][0] = m[j][1] = -INFINITY;
+      less[j][0] = less[j][1] = 0.f;
+      l[j][0] = l[j][1] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int z = 0; z < 4; ++z) o[i][j][z] = 0.f;
+    }
+  }
 };
 
 // N times 16 keys: s[n][j][2y + e] is the product of key 8y + g of chunk n with query 8j +
@@ -544,6 +557,169 @@ __device__ __forceinline__ void softmax_pv(WarpState<J>& st, float (&s)[N][J][4]
       }
 }
 
+__device__ __forceinline__ uint4 load16(const uint8_t* x) { return *reinterpret_cast<const uint4*>(x); }
+
+__device__ __forceinline__ uint32_t word_of(const uint4& u, int c) {
+  return c == 0 ? u.x : c == 1 ? u.y : c == 2 ? u.z : u.w;
+}
+
+// The pages of one CTA on their way into the ring: warp 0 holds the page ids, 32 at a time
+// and 32 ahead, and one lane issues the copies.
+struct PageFeed {
+  const int32_t* ids_of;
+  int ids, ids_next, h, np;
+
+  __device__ PageFeed(const AttnParams4& p, int b, int head, int first, int pages, int lane, bool mine)
+      : ids_of(p.table + static_cast<int64_t>(b) * p.max_pages + first), ids(0), ids_next(0), h(head), np(pages) {
+    if (mine) {
+      if (lane < np) ids = ids_of[lane];
+      if (32 + lane < np) ids_next = ids_of[32 + lane];
+    }
+  }
+
+  // Page j (0, 1, 2, ...) into slot j % depth; the whole of warp 0 calls it.
+  __device__ __forceinline__ void issue(const AttnParams4& p, uint8_t* ring, uint64_t* full, int depth, int j,
+                                        int lane) {
+    if (j > 0 && (j & 31) == 0) {
+      ids = ids_next;
+      if (j + 32 + lane < np) ids_next = ids_of[j + 32 + lane];
+    }
+    const int page = __shfl_sync(0xffffffffu, ids, j & 31);
+    const int slot = j % depth;
+    if (page >= 0 && page < p.num_pages) {
+      if (lane == 0) {
+        mbar_expect_tx(full + slot, kBlock);
+        bulk_load(ring + slot * kBlock, p.pool + (static_cast<int64_t>(page) * p.heads + h) * kBlock,
+                  kBlock, full + slot);
+      }
+    } else {  // no such page: steps of 0 make its tokens read as zeros
+      for (int i = lane; i < (kBlock - kKsOff) / 16; i += 32)
+        *reinterpret_cast<uint4*>(ring + slot * kBlock + kKsOff + i * 16) = make_uint4(0, 0, 0, 0);
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) {
+        report_bad_page(p.status);
+        mbar_arrive(full + slot);
+      }
+    }
+  }
+};
+
+// Q fragments of rows row0 .. row0 + nrows - 1 (zeros behind): query 8j + g, channel pairs in
+// the permuted order.
+template <int J>
+__device__ __forceinline__ void load_q(const AttnParams4& p, int b, int h, int row0, int nrows, int g, int t,
+                                       uint32_t (&qf)[8][J][2]) {
+  const __nv_bfloat16* qb =
+      p.q + ((static_cast<int64_t>(b) * p.heads + h) * p.tokens + row0) * kHeadDim + 8 * t;
+#pragma unroll
+  for (int j = 0; j < J; ++j)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const uint4 x = 8 * j + g < nrows
+                          ? *reinterpret_cast<const uint4*>(qb + (8 * j + g) * kHeadDim + 32 * c)
+                          : make_uint4(0, 0, 0, 0);
+      uint32_t pr[4];
+      pairs_of(x, pr);
+      qf[2 * c][j][0] = pr[0];
+      qf[2 * c][j][1] = pr[1];
+      qf[2 * c + 1][j][0] = pr[2];
+      qf[2 * c + 1][j][1] = pr[3];
+    }
+}
+
+// This call's own keys (bf16), chunks of 16: `start`, start + step, ...
+template <int J>
+__device__ __forceinline__ void own_keys(const AttnParams4& p, WarpState<J>& st, const uint32_t (&qf)[8][J][2],
+                                         int b, int h, int row0, int nrows, int tv, int start, int step, int g,
+                                         int t) {
+  const int most = p.row_limit ? min(tv, max(p.row_limit[row0 + nrows - 1], 0)) : tv;
+  const int chunks = (most + 15) / 16;
+  const __nv_bfloat16* kb = p.k + (static_cast<int64_t>(b) * p.heads + h) * p.tokens * kHeadDim;
+  const __nv_bfloat16* vb = p.v + (static_cast<int64_t>(b) * p.tokens * p.heads + h) * kHeadDim;
+  const int64_t v_st = static_cast<int64_t>(p.heads) * kHeadDim;
+  for (int ch = start; ch < chunks; ch += step) {
+    float s[1][J][4];
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+#pragma unroll
+      for (int z = 0; z < 4; ++z) s[0][j][z] = 0.f;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      uint32_t lo[4], hi[4];
+      const int k0 = ch * 16 + g, k1 = k0 + 8;
+      const uint4 zero = make_uint4(0, 0, 0, 0);
+      pairs_of(k0 < tv ? *reinterpret_cast<const uint4*>(kb + static_cast<int64_t>(k0) * kHeadDim + 32 * c + 8 * t) : zero, lo);
+      pairs_of(k1 < tv ? *reinterpret_cast<const uint4*>(kb + static_cast<int64_t>(k1) * kHeadDim + 32 * c + 8 * t) : zero, hi);
+#pragma unroll
+      for (int z = 0; z < 2; ++z) {
+        const uint32_t a[4] = {lo[2 * z], hi[2 * z], lo[2 * z + 1], hi[2 * z + 1]};
+#pragma unroll
+        for (int j = 0; j < J; ++j) mma_16816(s[0][j], a, qf[2 * c + z][j][0], qf[2 * c + z][j][1]);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        int lim = tv;
+        if (p.row_limit) lim = min(tv, max(p.row_limit[min(row0 + 8 * j + 2 * t + e, p.tokens - 1)], 0));
+        if (ch * 16 + g >= lim) s[0][j][e] = -INFINITY;
+        if (ch * 16 + g + 8 >= lim) s[0][j][2 + e] = -INFINITY;
+      }
+    softmax_pv<J, 1>(st, s, p.scale_log2, [&](int, int c, int z, uint32_t (&a)[4]) {
+      uint32_t x[4];  // keys 2t, 2t + 1 (and 8 more), channels 32c + 4g + 2z + {0, 1}
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int kk = ch * 16 + (i >> 1) * 8 + 2 * t + (i & 1);
+        x[i] = kk < tv ? *reinterpret_cast<const uint32_t*>(vb + kk * v_st + 32 * c + 4 * g + 2 * z) : 0u;
+      }
+      a[0] = prmt(x[0], x[1], 0x5410);
+      a[1] = prmt(x[0], x[1], 0x7632);
+      a[2] = prmt(x[2], x[3], 0x5410);
+      a[3] = prmt(x[2], x[3], 0x7632);
+    });
+  }
+}
+
+// The CTAs of a cluster share out the output: rank r finishes channels [128 r / S, 128 (r + 1)
+// / S) of every row, adding the partial outputs up in rank order.
+__device__ __forceinline__ void join_ctas(const AttnParams4& p, const float (*cta_ml)[2], const float* cta_o, int b,
+                                          int h, int row0, int nrows, int rank, int S, int threads) {
+  const int per = kHeadDim / S / 4;  // of 4 channels each
+  for (int i = threadIdx.x; i < nrows * per; i += threads) {
+    const int row = i / per, ch = rank * (kHeadDim / S) + (i % per) * 4;
+    float2 ml[kMaxSplits];
+    float4 x[kMaxSplits];
+#pragma unroll
+    for (int r = 0; r < kMaxSplits; ++r) {
+      const int from = r < S ? r : rank;  // past the last CTA: anything, with weight 0
+      ml[r] = peer_f32x2(peer_of(&cta_ml[row][0], from));
+      x[r] = peer_f32x4(peer_of(cta_o + row * kHeadDim + ch, from));
+    }
+    float m = -INFINITY, l = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int r = 0; r < kMaxSplits; ++r)
+      if (r < S) m = fmaxf(m, ml[r].x);
+#pragma unroll
+    for (int r = 0; r < kMaxSplits; ++r)
+      if (r < S) {
+        // m = -inf: no key, weight 0 — or scores that were all NaN, whose NaN in l has to stay
+        const float f = ml[r].x == -INFINITY ? 0.f : ex2_approx(ml[r].x - m);
+        l += ml[r].x == -INFINITY ? ml[r].y : f * ml[r].y;
+        acc.x = fmaf(f, x[r].x, acc.x);
+        acc.y = fmaf(f, x[r].y, acc.y);
+        acc.z = fmaf(f, x[r].z, acc.z);
+        acc.w = fmaf(f, x[r].w, acc.w);
+      }
+    const float inv = 1.f / l;
+    *reinterpret_cast<uint2*>(
+        p.out + ((static_cast<int64_t>(b) * p.tokens + row0 + row) * p.heads + h) * kHeadDim + ch) =
+        make_uint2(bf16_pair(acc.x * inv, acc.y * inv), bf16_pair(acc.z * inv, acc.w * inv));
+  }
+}
+
 template <int J>
 __global__ void __launch_bounds__(kThreads, AttnShape<J>::kCtas) kv4_attn_kernel(const AttnParams4 p) {
   using Shape = AttnShape<J>;
@@ -585,123 +761,16 @@ __global__ void __launch_bounds__(kThreads, AttnShape<J>::kCtas) kv4_attn_kernel
   }
   __syncthreads();
 
-  // Warp 0 keeps the ring filled: page ids by 32 at a time, one lane issues.
-  const int32_t* ids_of = p.table + static_cast<int64_t>(b) * p.max_pages + first;
-  int ids = 0, ids_next = 0;
-  if (warp == 0) {
-    if (lane < np) ids = ids_of[lane];
-    if (32 + lane < np) ids_next = ids_of[32 + lane];
-  }
-  auto issue = [&](int j) {  // warp 0, j = 0, 1, 2, ...
-    if (j > 0 && (j & 31) == 0) {
-      ids = ids_next;
-      if (j + 32 + lane < np) ids_next = ids_of[j + 32 + lane];
-    }
-    const int page = __shfl_sync(0xffffffffu, ids, j & 31);
-    const int slot = j % kRing;
-    if (page >= 0 && page < p.num_pages) {
-      if (lane == 0) {
-        mbar_expect_tx(full + slot, kBlock);
-        bulk_load(ring + slot * kBlock, p.pool + (static_cast<int64_t>(page) * p.heads + h) * kBlock,
-                  kBlock, full + slot);
-      }
-    } else {  // no such page: steps of 0 make its tokens read as zeros
-      for (int i = lane; i < (kBlock - kKsOff) / 16; i += 32)
-        *reinterpret_cast<uint4*>(ring + slot * kBlock + kKsOff + i * 16) = make_uint4(0, 0, 0, 0);
-      fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) {
-        report_bad_page(p.status);
-        mbar_arrive(full + slot);
-      }
-    }
-  };
+  PageFeed feed(p, b, h, first, np, lane, warp == 0);
   int issued = 0;
   if (warp == 0)
-    for (; issued < np && issued < kRing; ++issued) issue(issued);
+    for (; issued < np && issued < kRing; ++issued) feed.issue(p, ring, full, kRing, issued, lane);
 
-  // Q fragments: query 8j + g (zeros behind the last row), channel pairs in the permuted order
   uint32_t qf[8][J][2];
-  {
-    const __nv_bfloat16* qb =
-        p.q + ((static_cast<int64_t>(b) * p.heads + h) * p.tokens + row0) * kHeadDim + 8 * t;
-#pragma unroll
-    for (int j = 0; j < J; ++j)
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const uint4 x = 8 * j + g < nrows
-                            ? *reinterpret_cast<const uint4*>(qb + (8 * j + g) * kHeadDim + 32 * c)
-                            : make_uint4(0, 0, 0, 0);
-        uint32_t pr[4];
-        pairs_of(x, pr);
-        qf[2 * c][j][0] = pr[0];
-        qf[2 * c][j][1] = pr[1];
-        qf[2 * c + 1][j][0] = pr[2];
-        qf[2 * c + 1][j][1] = pr[3];
-      }
-  }
+  load_q<J>(p, b, h, row0, nrows, g, t, qf);
   WarpState<J> st;
-#pragma unroll
-  for (int j = 0; j < J; ++j) {
-    st.m[j][0] = st.m[j][1] = -INFINITY;
-    st.less[j][0] = st.less[j][1] = 0.f;
-    st.l[j][0] = st.l[j][1] = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-#pragma unroll
-      for (int z = 0; z < 4; ++z) st.o[i][j][z] = 0.f;
-  }
-
-  // ---- this call's own keys (bf16), 16 at a time, dealt out over CTAs and warps
-  {
-    const int most = p.row_limit ? min(tv, max(p.row_limit[row0 + nrows - 1], 0)) : tv;
-    const int chunks = (most + 15) / 16;
-    const __nv_bfloat16* kb = p.k + (static_cast<int64_t>(b) * p.heads + h) * p.tokens * kHeadDim;
-    const __nv_bfloat16* vb = p.v + (static_cast<int64_t>(b) * p.tokens * p.heads + h) * kHeadDim;
-    const int64_t v_st = static_cast<int64_t>(p.heads) * kHeadDim;
-    for (int ch = rank + S * warp; ch < chunks; ch += kWarps * S) {
-      float s[1][J][4];
-#pragma unroll
-      for (int j = 0; j < J; ++j)
-#pragma unroll
-        for (int z = 0; z < 4; ++z) s[0][j][z] = 0.f;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t lo[4], hi[4];
-        const int k0 = ch * 16 + g, k1 = k0 + 8;
-        const uint4 zero = make_uint4(0, 0, 0, 0);
-        pairs_of(k0 < tv ? *reinterpret_cast<const uint4*>(kb + static_cast<int64_t>(k0) * kHeadDim + 32 * c + 8 * t) : zero, lo);
-        pairs_of(k1 < tv ? *reinterpret_cast<const uint4*>(kb + static_cast<int64_t>(k1) * kHeadDim + 32 * c + 8 * t) : zero, hi);
-#pragma unroll
-        for (int z = 0; z < 2; ++z) {
-          const uint32_t a[4] = {lo[2 * z], hi[2 * z], lo[2 * z + 1], hi[2 * z + 1]};
-#pragma unroll
-          for (int j = 0; j < J; ++j) mma_16816(s[0][j], a, qf[2 * c + z][j][0], qf[2 * c + z][j][1]);
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < J; ++j)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          int lim = tv;
-          if (p.row_limit) lim = min(tv, max(p.row_limit[min(row0 + 8 * j + 2 * t + e, p.tokens - 1)], 0));
-          if (ch * 16 + g >= lim) s[0][j][e] = -INFINITY;
-          if (ch * 16 + g + 8 >= lim) s[0][j][2 + e] = -INFINITY;
-        }
-      softmax_pv<J, 1>(st, s, p.scale_log2, [&](int, int c, int z, uint32_t (&a)[4]) {
-        uint32_t x[4];  // keys 2t, 2t + 1 (and 8 more), channels 32c + 4g + 2z + {0, 1}
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int kk = ch * 16 + (i >> 1) * 8 + 2 * t + (i & 1);
-          x[i] = kk < tv ? *reinterpret_cast<const uint32_t*>(vb + kk * v_st + 32 * c + 4 * g + 2 * z) : 0u;
-        }
-        a[0] = prmt(x[0], x[1], 0x5410);
-        a[1] = prmt(x[0], x[1], 0x7632);
-        a[2] = prmt(x[2], x[3], 0x5410);
-        a[3] = prmt(x[2], x[3], 0x7632);
-      });
-    }
-  }
+  st.clear();
+  own_keys<J>(p, st, qf, b, h, row0, nrows, tv, rank + S * warp, kWarps * S, g, t);
 
   // ---- the prefix's pages
   const uint32_t key_sel = (g & 1) ? 0x3232 : 0x1010;  // token g's step of a pair, twice
@@ -716,20 +785,18 @@ __global__ void __launch_bounds__(kThreads, AttnShape<J>::kCtas) kv4_attn_kernel
       // chunk n of this warp: octets 2n and 2n + 1 from `at` on
       const uint8_t* at = ring + slot * kBlock + warp * (kChunks * 2 * kOctetBytes) + lane * 16;
       const uint8_t* steps = ring + slot * kBlock + kKsOff + warp * (kChunks * 2 * kOctetStepBytes);
-      auto load = [](const uint8_t* x) { return *reinterpret_cast<const uint4*>(x); };
-      auto word = [](const uint4& u, int c) { return c == 0 ? u.x : c == 1 ? u.y : c == 2 ? u.z : u.w; };
       float s[kChunks][J][4];
 #pragma unroll
       for (int n = 0; n < kChunks; ++n) {
         uint4 kw[2], ks[2];
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
-          kw[y] = load(at + (2 * n + y) * kOctetBytes);
-          ks[y] = load(steps + (2 * n + y) * kOctetStepBytes + (g >> 1) * 16);
+          kw[y] = load16(at + (2 * n + y) * kOctetBytes);
+          ks[y] = load16(steps + (2 * n + y) * kOctetStepBytes + (g >> 1) * 16);
         }
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          const uint32_t w0 = word(kw[0], c), w1 = word(kw[1], c), p0 = word(ks[0], c), p1 = word(ks[1], c);
+          const uint32_t w0 = word_of(kw[0], c), w1 = word_of(kw[1], c), p0 = word_of(ks[0], c), p1 = word_of(ks[1], c);
           const uint32_t s0 = prmt(p0, p0, key_sel), s1 = prmt(p1, p1, key_sel);
           const uint32_t l0 = less_of(s0), l1 = less_of(s1);
 #pragma unroll
@@ -760,8 +827,8 @@ __global__ void __launch_bounds__(kThreads, AttnShape<J>::kCtas) kv4_attn_kernel
         if (c == 0 && z == 0) {
 #pragma unroll
           for (int y = 0; y < 2; ++y) {
-            vw[y] = load(at + kVOff + (2 * n + y) * kOctetBytes);
-            vs[y] = load(steps + (kVsOff - kKsOff) + (2 * n + y) * kOctetStepBytes + t * 16);
+            vw[y] = load16(at + kVOff + (2 * n + y) * kOctetBytes);
+            vs[y] = load16(steps + (kVsOff - kKsOff) + (2 * n + y) * kOctetStepBytes + t * 16);
             if (!whole) {  // nor a V step that could be NaN
               const int key = 16 * n + 8 * y + 2 * t;
               const uint32_t keep = (key < left ? 0x0000ffffu : 0u) | (key + 1 < left ? 0xffff0000u : 0u);
@@ -772,8 +839,8 @@ __global__ void __launch_bounds__(kThreads, AttnShape<J>::kCtas) kv4_attn_kernel
             }
           }
         }
-        const uint32_t v0 = word(vw[0], c), v1 = word(vw[1], c);
-        const uint32_t s0 = word(vs[0], c), s1 = word(vs[1], c);
+        const uint32_t v0 = word_of(vw[0], c), v1 = word_of(vw[1], c);
+        const uint32_t s0 = word_of(vs[0], c), s1 = word_of(vs[1], c);
         const uint32_t l0 = less_of(s0), l1 = less_of(s1);
         a[0] = expand_pair(v0, 2 * z, s0, l0);
         a[1] = expand_pair(v0, 2 * z + 1, s0, l0);
@@ -788,7 +855,8 @@ __global__ void __launch_bounds__(kThreads, AttnShape<J>::kCtas) kv4_attn_kernel
       const int prev = slot == 0 ? kRing - 1 : slot - 1;
       ok = warp_wait(empty + prev, slot == 0 ? parity ^ 1 : parity, abort_flag);
       if (!ok) break;
-      issue(issued++);
+      feed.issue(p, ring, full, kRing, issued, lane);
+      ++issued;
     }
     if (++slot == kRing) {
       slot = 0;
@@ -861,39 +929,214 @@ __global__ void __launch_bounds__(kThreads, AttnShape<J>::kCtas) kv4_attn_kernel
     }
   }
   if (S == 1) return;
-  // ---- join the CTAs: rank r finishes channels [128 r / S, 128 (r + 1) / S) of every row
+  // ---- join the CTAs
   cluster_barrier();
-  const int per = kHeadDim / S / 4;  // of 4 channels each
-  for (int i = threadIdx.x; i < nrows * per; i += kThreads) {
-    const int row = i / per, ch = rank * (kHeadDim / S) + (i % per) * 4;
-    float2 ml[kMaxSplits];
-    float4 x[kMaxSplits];
-#pragma unroll
-    for (int r = 0; r < kMaxSplits; ++r) {
-      const int from = r < S ? r : rank;  // past the last CTA: anything, with weight 0
-      ml[r] = peer_f32x2(peer_of(&cta_ml[row][0], from));
-      x[r] = peer_f32x4(peer_of(cta_o + row * kHeadDim + ch, from));
-    }
-    float m = -INFINITY, l = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int r = 0; r < kMaxSplits; ++r)
-      if (r < S) m = fmaxf(m, ml[r].x);
-#pragma unroll
-    for (int r = 0; r < kMaxSplits; ++r)
-      if (r < S) {
-        const float f = ml[r].x == -INFINITY ? 0.f : ex2_approx(ml[r].x - m);
-        l += ml[r].x == -INFINITY ? ml[r].y : f * ml[r].y;
-        acc.x = fmaf(f, x[r].x, acc.x);
-        acc.y = fmaf(f, x[r].y, acc.y);
-        acc.z = fmaf(f, x[r].z, acc.z);
-        acc.w = fmaf(f, x[r].w, acc.w);
-      }
-    const float inv = 1.f / l;
-    *reinterpret_cast<uint2*>(
-        p.out + ((static_cast<int64_t>(b) * p.tokens + row0 + row) * p.heads + h) * kHeadDim + ch) =
-        make_uint2(bf16_pair(acc.x * inv, acc.y * inv), bf16_pair(acc.z * inv, acc.w * inv));
+  join_ctas(p, cta_ml, cta_o, b, h, row0, nrows, rank, S, kThreads);
+  cluster_barrier();  // no CTA leaves while another reads its shared memory
+}
+
+// ------------------------------------------------------------------ attention of more rows
+// 64 query rows per CTA: the kernel above repeats the expansion for every 16 rows.  Here each
+// of 4 warps expands a quarter of the page into shared memory, once, in the order of the
+// matrix fragments (a lane writes and reads 16 bytes, a warp 512 in a row), and then takes
+// its own 16 rows over the whole page.  No join of warps; clusters split the pages as above.
+// Bound by the latency of a page's two phases, with 3 CTAs per SM to fill the gaps: 1.27 us
+// of an SM per page and head for 64 rows, 1.0 us for 17, against 0.38 us for each 16 rows
+// above.  (Two buffers and one barrier per page at 2 CTAs per SM: 1.5 us; all 64 keys of a
+// page in one softmax step: 1.30 us.)
+constexpr int kTileRows = 64;
+constexpr int kTileWarps = 4;
+constexpr int kTileThreads = 32 * kTileWarps;
+constexpr int kTileRing = 3;
+constexpr int kTileCtas = 3;                       // per SM, by registers
+constexpr int kFragBytes = 512;                    // one fragment of a warp
+constexpr int kWideBytes = 4 * 8 * kFragBytes;     // a page's K or V: 4 chunks of 8 fragments
+constexpr int kTileSmem = kTileRing * kBlock + 2 * kWideBytes;
+static_assert(2 * kWideBytes >= kTileRows * kHeadDim * 4, "the CTA's outputs take the fragments' place");
+
+__global__ void __launch_bounds__(kTileThreads, kTileCtas) kv4_attn_tile_kernel(const AttnParams4 p) {
+  constexpr int J = 2;
+  extern __shared__ __align__(128) uint8_t ring[];
+  uint8_t* wide_k = ring + kTileRing * kBlock;
+  uint8_t* wide_v = wide_k + kWideBytes;
+  float* cta_o = reinterpret_cast<float*>(wide_k);  // after the last page: [kTileRows][128]
+  __shared__ __align__(8) float cta_ml[kTileRows][2];
+  __shared__ __align__(8) uint64_t full[kTileRing];
+  __shared__ int abort_word;
+  volatile int* abort_flag = &abort_word;
+
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int g = lane >> 2, t = lane & 3;
+  const int S = p.splits;
+  const int rank = S > 1 ? static_cast<int>(cluster_rank()) : 0;
+  const int item = blockIdx.x / S;
+  const int mt = item % p.row_tiles;
+  const int h = (item / p.row_tiles) % p.heads;
+  const int b = item / (p.row_tiles * p.heads);
+  const int cta_row0 = mt * kTileRows, cta_rows = min(kTileRows, p.tokens - cta_row0);
+  const int row0 = cta_row0 + warp * 8 * J;                   // this warp's rows
+  const int nrows = min(8 * J, p.tokens - row0);              // <= 0: none, it only expands
+
+  const int pv = p.desc ? min(max(p.desc[b].prefix_valid, 0), p.prefix_len) : p.prefix_len;
+  const int tv = p.desc ? min(max(p.desc[b].target_valid, 0), p.tokens) : p.tokens;
+  const int pages = (pv + kPage - 1) / kPage;
+  const int first = static_cast<int>(static_cast<int64_t>(pages) * rank / S);
+  const int np = static_cast<int>(static_cast<int64_t>(pages) * (rank + 1) / S) - first;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kTileRing; ++i) mbar_init(full + i, 1);
+    abort_word = 0;
+    fence_barrier_init();
+    fence_proxy_async();
   }
+  __syncthreads();
+  PageFeed feed(p, b, h, first, np, lane, warp == 0);
+  int issued = 0;
+  if (warp == 0)
+    for (; issued < np && issued < kTileRing; ++issued) feed.issue(p, ring, full, kTileRing, issued, lane);
+
+  uint32_t qf[8][J][2];
+  load_q<J>(p, b, h, row0, nrows, g, t, qf);
+  WarpState<J> st;
+  st.clear();
+  if (nrows > 0) own_keys<J>(p, st, qf, b, h, row0, nrows, tv, rank, S, g, t);
+
+  const uint32_t key_sel = (g & 1) ? 0x3232 : 0x1010;  // token g's step of a pair, twice
+  bool ok = true;
+  int slot = 0;
+  uint32_t parity = 0;
+  for (int j = 0; j < np; ++j) {
+    ok = warp_wait(full + slot, parity, abort_flag);
+    // every warp is done with the page before
+    ok = __syncthreads_and(ok);
+    if (!ok) break;
+    const int left = pv - (first + j) * kPage;  // valid keys of this page (and behind it)
+    {  // expand chunk `warp`
+      const uint8_t* at = ring + slot * kBlock + warp * (2 * kOctetBytes) + lane * 16;
+      const uint8_t* steps = ring + slot * kBlock + kKsOff + warp * (2 * kOctetStepBytes);
+      uint4 kw[2], ks[2], vw[2], vs[2];
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        kw[y] = load16(at + y * kOctetBytes);
+        ks[y] = load16(steps + y * kOctetStepBytes + (g >> 1) * 16);
+        vw[y] = load16(at + kVOff + y * kOctetBytes);
+        vs[y] = load16(steps + (kVsOff - kKsOff) + y * kOctetStepBytes + t * 16);
+        const int key = 16 * warp + 8 * y + 2 * t;
+        if (key + 1 >= left) {  // behind the last token: no V step that could be NaN
+          const uint32_t keep = key < left ? 0x0000ffffu : 0u;
+          vs[y].x &= keep;
+          vs[y].y &= keep;
+          vs[y].z &= keep;
+          vs[y].w &= keep;
+        }
+      }
+      uint8_t* to = wide_k + warp * 8 * kFragBytes + lane * 16;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t s0 = word_of(ks[0], c), s1 = word_of(ks[1], c);
+        s0 = prmt(s0, s0, key_sel);
+        s1 = prmt(s1, s1, key_sel);
+        const uint32_t w0 = word_of(kw[0], c), w1 = word_of(kw[1], c), l0 = less_of(s0), l1 = less_of(s1);
+        const uint32_t u0 = word_of(vs[0], c), u1 = word_of(vs[1], c);
+        const uint32_t v0 = word_of(vw[0], c), v1 = word_of(vw[1], c), m0 = less_of(u0), m1 = less_of(u1);
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {
+          *reinterpret_cast<uint4*>(to + (2 * c + z) * kFragBytes) =
+              make_uint4(expand_pair(w0, 2 * z, s0, l0), expand_pair(w1, 2 * z, s1, l1),
+                         expand_pair(w0, 2 * z + 1, s0, l0), expand_pair(w1, 2 * z + 1, s1, l1));
+          *reinterpret_cast<uint4*>(to + kWideBytes + (2 * c + z) * kFragBytes) =
+              make_uint4(expand_pair(v0, 2 * z, u0, m0), expand_pair(v0, 2 * z + 1, u0, m0),
+                         expand_pair(v1, 2 * z, u1, m1), expand_pair(v1, 2 * z + 1, u1, m1));
+        }
+      }
+    }
+    __syncthreads();  // the page is expanded, and its slot is free
+    if (warp == 0 && issued < np) {
+      feed.issue(p, ring, full, kTileRing, issued, lane);
+      ++issued;
+    }
+    if (nrows > 0) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {  // 32 keys at a time
+        if (32 * half >= left) break;
+        const uint8_t* fk = wide_k + half * 16 * kFragBytes + lane * 16;
+        const uint8_t* fv = wide_v + half * 16 * kFragBytes + lane * 16;
+        float s[2][J][4];
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int f = 0; f < 8; ++f) {
+            const uint4 x = load16(fk + (n * 8 + f) * kFragBytes);
+            const uint32_t a[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+            for (int i = 0; i < J; ++i) {
+              const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+              if (f == 0) mma_16816(s[n][i], a, qf[0][i][0], qf[0][i][1], zero);
+              else mma_16816(s[n][i], a, qf[f][i][0], qf[f][i][1]);
+            }
+          }
+        if (left < 32 * half + 32) {  // no score behind the last token
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int i = 0; i < J; ++i)
+#pragma unroll
+              for (int z = 0; z < 4; ++z)
+                if (32 * half + 16 * n + 8 * (z >> 1) + g >= left) s[n][i][z] = -INFINITY;
+        }
+        softmax_pv<J, 2>(st, s, p.scale_log2, [&](int n, int c, int z, uint32_t (&a)[4]) {
+          const uint4 x = load16(fv + (n * 8 + 2 * c + z) * kFragBytes);
+          a[0] = x.x;
+          a[1] = x.y;
+          a[2] = x.z;
+          a[3] = x.w;
+        });
+      }
+    }
+    if (++slot == kTileRing) {
+      slot = 0;
+      parity ^= 1;
+    }
+  }
+  if (!ok) {
+    if (lane == 0) {
+      *abort_flag = 1;
+      if (p.status) atomicCAS(p.status, 0, 1);
+    }
+    if (warp == 0)  // copies in flight land before the CTA leaves
+      for (int j = max(issued - kTileRing, 0); j < issued; ++j)
+        mbar_wait(full + j % kTileRing, (j / kTileRing) & 1);
+  }
+  __syncthreads();  // the fragments are read; their place takes the outputs
+
+#pragma unroll
+  for (int j = 0; j < J; ++j)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int q = 8 * j + 2 * t + e;
+      float l = st.l[j][e];
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+      if (q >= nrows) continue;
+      const float f = S == 1 ? 1.f / l : 1.f;  // no key: 0 * (1 / 0) = NaN
+      if (S > 1 && g == 0) {
+        cta_ml[warp * 8 * J + q][0] = st.m[j][e];
+        cta_ml[warp * 8 * J + q][1] = l;
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const float4 x = make_float4(st.o[2 * c][j][e] * f, st.o[2 * c][j][2 + e] * f, st.o[2 * c + 1][j][e] * f,
+                                     st.o[2 * c + 1][j][2 + e] * f);
+        if (S == 1)
+          *reinterpret_cast<uint2*>(p.out + ((static_cast<int64_t>(b) * p.tokens + row0 + q) * p.heads + h) * kHeadDim +
+                                    32 * c + 4 * g) = make_uint2(bf16_pair(x.x, x.y), bf16_pair(x.z, x.w));
+        else
+          *reinterpret_cast<float4*>(cta_o + (warp * 8 * J + q) * kHeadDim + 32 * c + 4 * g) = x;
+      }
+    }
+  if (S == 1) return;
+  cluster_barrier();
+  join_ctas(p, cta_ml, cta_o, b, h, cta_row0, cta_rows, rank, S, kTileThreads);
   cluster_barrier();  // no CTA leaves while another reads its shared memory
 }
 
@@ -945,18 +1188,22 @@ int pick_splits(int64_t items, int prefix_len, int resident) {
   return s;
 }
 
-template <int J>
-int launch_few_rows_of(AttnParams4 p, int batch, cudaStream_t stream) {
-  using Shape = AttnShape<J>;
-  p.row_tiles = (p.tokens + Shape::kRows - 1) / Shape::kRows;
+template <typename Kernel>
+int launch_rows(Kernel kernel, AttnParams4 p, int rows, int resident, int threads, int smem, int batch,
+                cudaStream_t stream) {
+  p.row_tiles = (p.tokens + rows - 1) / rows;
   const int64_t items = static_cast<int64_t>(batch) * p.heads * p.row_tiles;
-  p.splits = pick_splits(items, p.prefix_len, Shape::kCtas);
+  p.splits = pick_splits(items, p.prefix_len, resident);
   if (items * p.splits > 0x7fffffff) return B200_ERR_INVALID;
-  static_assert(Shape::kSmem <= 47 * 1024, "no attribute needed");
+  if (smem > 48 * 1024 &&
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
+    cudaGetLastError();
+    return B200_ERR_CUDA;
+  }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(items * p.splits));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = Shape::kSmem;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -965,8 +1212,14 @@ int launch_few_rows_of(AttnParams4 p, int batch, cudaStream_t stream) {
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kv4_attn_kernel<J>, p);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
   return e == cudaSuccess && cudaGetLastError() == cudaSuccess ? B200_OK : B200_ERR_CUDA;
+}
+
+template <int J>
+int launch_few_rows_of(const AttnParams4& p, int batch, cudaStream_t stream) {
+  using Shape = AttnShape<J>;
+  return launch_rows(kv4_attn_kernel<J>, p, Shape::kRows, Shape::kCtas, kThreads, Shape::kSmem, batch, stream);
 }
 
 int launch_few_rows(const b200_kv4_view& c, const void* q, const void* k, const void* v, int batch,
@@ -989,20 +1242,23 @@ int launch_few_rows(const b200_kv4_view& c, const void* q, const void* k, const 
   p.tokens = tokens;
   p.prefix_len = prefix_len;
   p.scale_log2 = scale * 1.4426950408889634f;
-  return tokens <= 8 ? launch_few_rows_of<1>(p, batch, stream) : launch_few_rows_of<2>(p, batch, stream);
+  if (tokens <= 8) return launch_few_rows_of<1>(p, batch, stream);
+  // 32 heads, 33 rows against 32: 16 sequences over 512 tokens, 46 us here and 50 us there;
+  // 64 rows: 54 and 65 us, over 10.6k tokens 732 and 992 us, one sequence 55 and 81 us
+  if (tokens <= 32) return launch_few_rows_of<2>(p, batch, stream);
+  return launch_rows(kv4_attn_tile_kernel, p, kTileRows, kTileCtas, kTileThreads, kTileSmem, batch, stream);
 }
 
 size_t round256(size_t x) { return (x + 255) / 256 * 256; }
 
-// Whether the pages are read by the few-row kernel or expanded for the tensor-core kernel.
-// Per page, head and 16 rows the former takes 0.38 us of an SM; the latter takes the
-// expansion's 0.6 KB per token and head at HBM rate, and its 256-row tiles cost the same for
-// 1 row.  64 against 65 rows: 992 and 1205 us for 16 x 32 heads over 10.6k tokens, 140 and
-// 149 us for 4 x 32 over 5k; 80 rows: 1232 and 1202 us, 176 and 151 us.  With few heads in
-// all the dense tiles leave SMs idle, and the pages win up to 128 rows: 32 heads, 128 rows,
-// 17.4 and 17.8 us over 512 tokens, 148 and 192 us over 10.6k; 160 rows: 21.6 and 20.1 us.
-bool few_rows(int64_t batch, int64_t heads, int target_len) {
-  return target_len <= 64 || (target_len <= 128 && batch * heads <= 64);
+// Whether the pages are read by the kernels above or expanded for the tensor-core kernel,
+// whose 256-row tiles cost the same for 1 row, behind 0.66 KB per token and head at HBM rate.
+// Pages and dense, in us: 64 rows, 16 x 32 heads over 10.6k tokens 732 and 1186, 4 x 32 over
+// 5k 105 and 150, over 500 22 and 23; 128 rows 1432 and 1189, 202 and 150, 35 and 23.  With
+// few heads in all the dense tiles leave SMs idle: 32 heads, 128 rows, 121 and 192 over
+// 10.6k, 16.2 and 18.1 over 512 — but 17 and 13 over 64, where the own keys weigh more.
+bool few_rows(int64_t batch, int64_t heads, int target_len, int prefix_len) {
+  return target_len <= 64 || (target_len <= 128 && batch * heads <= 64 && prefix_len / 4 >= target_len);
 }
 
 size_t dense_bytes(int batch, int heads, int prefix_len) {
@@ -1098,7 +1354,7 @@ extern "C" int b200_kv4_copy_pages(void* pool, int32_t layers, int64_t layer_str
 extern "C" int b200_kv4_attention_workspace_bytes(int32_t batch, int32_t heads, int32_t target_len,
                                                   int32_t prefix_len, size_t* bytes) {
   if (!bytes || batch < 0 || heads < 0 || target_len < 0 || prefix_len < 0) return B200_ERR_INVALID;
-  *bytes = few_rows(batch, heads, target_len)
+  *bytes = few_rows(batch, heads, target_len, prefix_len)
                ? 0
                : 2 * dense_bytes(batch, heads, prefix_len) + B200_ATTN_SPLIT_WORKSPACE_BYTES;
   return B200_OK;
@@ -1124,7 +1380,7 @@ extern "C" int b200_kv4_joint_attention(const b200_kv4_view* c, const void* q_ro
     if (!al16(ptr)) return B200_ERR_INVALID;
   if (!(scale > 0.f) || !std::isfinite(scale)) return B200_ERR_INVALID;
   auto stream = static_cast<cudaStream_t>(stream_);
-  if (few_rows(batch, heads, target_len))
+  if (few_rows(batch, heads, target_len, prefix_len))
     return launch_few_rows(*c, q_rot, k_rot, v, batch, heads, target_len, prefix_len, desc, row_limit,
                            scale, out, status, stream);
   size_t need = 0;

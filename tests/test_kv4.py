@@ -141,7 +141,8 @@ def test_attention_refuses_bad_arguments():
     # many rows expand the pages into a workspace
     need = b200attn.kv4_workspace_bytes(1, 2, 200, 128)
     assert need >= 2 * 2 * 128 * D * 2 and b200attn.kv4_workspace_bytes(4, 32, 65, 128) > need
-    assert b200attn.kv4_workspace_bytes(4, 32, 64, 128) == b200attn.kv4_workspace_bytes(1, 2, 128, 128) == 0
+    assert b200attn.kv4_workspace_bytes(4, 32, 64, 128) == b200attn.kv4_workspace_bytes(1, 2, 128, 512) == 0
+    assert b200attn.kv4_workspace_bytes(1, 2, 128, 511) > 0
     assert attend(t=200) == b200attn.ERR_WORKSPACE
     assert attend(t=200, ws=256, n=need - 1) == b200attn.ERR_WORKSPACE
 
@@ -343,7 +344,7 @@ def test_bad_pages_are_left_out_and_reported(cuda):
     kk, _ = b200attn.kv4_load(pool, broken, None, 200, status=status)
     assert status.item() == b200attn.KV4_STATUS_BAD_PAGE
     assert torch.equal(kk[0, :, 64:192], torch.zeros_like(kk[0, :, 64:192]))
-    for t in (5, 150):  # both forms of the attention: such tokens count as keys of zeros
+    for t in (5, 40, 150):  # the three forms of the attention: such tokens count as keys of zeros
         q, ko = (torch.randn(1, 2, t, D, generator=g).bfloat16().to(cuda) for _ in range(2))
         vo = torch.randn(1, t, 2, D, generator=g).bfloat16().to(cuda)
         status.zero_()
@@ -382,6 +383,8 @@ ATTEND = [  # (prefix lengths, tokens, target_valid, heads, causal)
     ([17, 1000, 300], 16, [16, 9, 1], 2, True), ([2000], 17, [17], 3, False),
     ([100, 7], 37, [37, 20], 5, True), ([5000], 64, [64], 1, True),
     ([129, 30], 65, [65, 40], 2, True), ([700, 0], 300, [300, 299], 3, False),
+    ([33], 33, [33], 2, True), ([520, 3, 0], 48, [48, 1, 0], 3, False), ([600, 2], 100, [100, 99], 2, True),
+    ([3000], 50, [50], 1, False), ([1500, 1500], 128, [128, 60], 1, True),
     ([300, 64, 1], 129, [129, 70, 0], 2, True), ([70] * 5, 66, [66, 65, 3, 1, 0], 16, True),
     ([0, 0], 5, [5, 0], 2, True), ([0, 64], 130, [0, 130], 1, False),
 ]
