@@ -698,7 +698,7 @@ def kv4_joint_attention(q_rot, k_rot, v, pool, page_table, prefix_len: int, desc
         _expect(row_limit, "row_limit", torch.int32, (t,), dev)
     with _Launch(pool, stream) as st:
         if out is None:
-            out = q_rot.new_empty((b, t, h * d))
+            out = torch.empty((b, t, h * d), dtype=bf, device=dev)
         else:
             _expect(out, "out", bf, (b, t, h * d), dev)
         if workspace is None and t > 64:  # up to there it needs none

@@ -392,6 +392,7 @@ __global__ void __launch_bounds__(kLThreads, 2)
     // ------------------------------------------------------------------ epilogue
     const int q = warp & 3;
     const int tr = q * 32 + lane;  // row of the tile = TMEM lane
+    const int mine = rows - q * 32;  // rows of this warp; <= 0: it only keeps the barriers going
     const uint32_t lane_off = static_cast<uint32_t>(q * 32) << 16;
     const float scale = p.scale ? p.scale[adapter] : 1.f;
     bool ok = mbar_wait(u_full, 0, abort_flag);
@@ -411,7 +412,7 @@ __global__ void __launch_bounds__(kLThreads, 2)
     auto u_chunk = [&](int r, int j) { return u_buf + (j >> 3) * kXBytes + r * 128 + (((j & 7) ^ (r & 7)) << 4); };
     if (ok) {
       if (C == 1) {
-        for (int c = 0; c < p.rp; c += 16) {
+        for (int c = 0; c < p.rp && mine > 0; c += 16) {
           uint32_t r[16];
           u_cols(c, r);
 #pragma unroll
@@ -424,7 +425,7 @@ __global__ void __launch_bounds__(kLThreads, 2)
           }
         }
       } else {
-        for (int c = 0; c < p.rp; c += 16) {
+        for (int c = 0; c < p.rp && mine > 0; c += 16) {
           uint32_t r[16];
           u_cols(c, r);
 #pragma unroll
@@ -509,22 +510,24 @@ __global__ void __launch_bounds__(kLThreads, 2)
       tc_fence_after();
       uint8_t* yt = ring + s * p.stage_bytes;
       uint4* yrow = reinterpret_cast<uint4*>(yt + tr * 128);
+      if (mine > 0) {
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        uint32_t r[32];
-        tmem_ld32(tmem_base + kAccCol + lane_off + (i & 1) * kTN + half * 32, r);
-        tmem_wait_ld();
+        for (int half = 0; half < 2; ++half) {
+          uint32_t r[32];
+          tmem_ld32(tmem_base + kAccCol + lane_off + (i & 1) * kTN + half * 32, r);
+          tmem_wait_ld();
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          uint4* at = yrow + ((half * 4 + j) ^ (tr & 7));
-          const uint4 v = *at;
-          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-          uint32_t o[4];
+          for (int j = 0; j < 4; ++j) {
+            uint4* at = yrow + ((half * 4 + j) ^ (tr & 7));
+            const uint4 v = *at;
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+            uint32_t o[4];
 #pragma unroll
-          for (int z = 0; z < 4; ++z)
-            o[z] = lora_pack(__uint_as_float(w[z] << 16) + __uint_as_float(r[8 * j + 2 * z]),
-                             __uint_as_float(w[z] & 0xffff0000u) + __uint_as_float(r[8 * j + 2 * z + 1]));
-          *at = make_uint4(o[0], o[1], o[2], o[3]);
+            for (int z = 0; z < 4; ++z)
+              o[z] = lora_pack(__uint_as_float(w[z] << 16) + __uint_as_float(r[8 * j + 2 * z]),
+                               __uint_as_float(w[z] & 0xffff0000u) + __uint_as_float(r[8 * j + 2 * z + 1]));
+            *at = make_uint4(o[0], o[1], o[2], o[3]);
+          }
         }
       }
       tc_fence_before();
@@ -534,14 +537,17 @@ __global__ void __launch_bounds__(kLThreads, 2)
       const int col = (n_first + i) * kTN + (lane & 7) * 8;
 #pragma unroll
       for (int pass = 0; pass < 8; ++pass) {
+        if (pass * 4 >= mine) break;
         const int rr = q * 32 + pass * 4 + (lane >> 3);
         const uint4 v = reinterpret_cast<const uint4*>(yt)[rr * 8 + ((lane & 7) ^ (rr & 7))];
         if (rr < rows && col < p.n)
           *reinterpret_cast<uint4*>(p.out + static_cast<int64_t>(row0 + rr) * p.ldo + col) = v;
       }
-      fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(empty2 + s);
+      if (i + NS < nb) {  // the stage takes another tile: after this warp's plain accesses to it
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(empty2 + s);
+      }
     }
     if (!ok && lane == 0) {
       *abort_flag = 1;
