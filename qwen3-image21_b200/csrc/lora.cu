@@ -533,15 +533,19 @@ __global__ void __launch_bounds__(kLThreads, 2)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(acc_empty + (i & 1));
-      // this warp's 32 rows: 4 rows of 128 bytes per pass
+      // this warp's rows: 4 rows of 128 bytes per pass
       const int col = (n_first + i) * kTN + (lane & 7) * 8;
-#pragma unroll
-      for (int pass = 0; pass < 8; ++pass) {
-        if (pass * 4 >= mine) break;
+      auto store4 = [&](int pass) {
         const int rr = q * 32 + pass * 4 + (lane >> 3);
         const uint4 v = reinterpret_cast<const uint4*>(yt)[rr * 8 + ((lane & 7) ^ (rr & 7))];
         if (rr < rows && col < p.n)
           *reinterpret_cast<uint4*>(p.out + static_cast<int64_t>(row0 + rr) * p.ldo + col) = v;
+      };
+      if (mine >= 32) {
+#pragma unroll
+        for (int pass = 0; pass < 8; ++pass) store4(pass);
+      } else {
+        for (int pass = 0; pass * 4 < mine; ++pass) store4(pass);
       }
       if (i + NS < nb) {  // the stage takes another tile: after this warp's plain accesses to it
         fence_proxy_async();
