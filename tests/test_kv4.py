@@ -412,3 +412,65 @@ def test_joint_attention(cuda, lengths, tokens, valid, heads, causal):
                                        row_limit=None if limit is None else limit.to(cuda), status=status)
     assert status.item() == 0
     check(got, q, ko, vo, values(dense[0]), values(dense[1]), list(zip(lengths, valid)), limit)
+
+
+@pytest.mark.gpu
+def test_pages_behind_32_bit_offsets(cuda):
+    """A pool of more than 4 GiB: its last pages are stored, read, copied and attended to."""
+    heads, pages = 32, 15000
+    pool = torch.zeros(pages, heads, BLOCK, dtype=torch.uint8, device=cuda)
+    table = i32(cuda, pages - 1, 0, pages - 2).view(1, 3)
+    g = torch.Generator().manual_seed(4)
+    k, v = (torch.randn(1, heads, 150, D, generator=g).bfloat16() for _ in range(2))
+    b200attn.kv4_store(k.to(cuda), v.to(cuda), pool, table)
+    b200attn.kv4_copy_pages(pool, [pages - 1], [pages - 3])
+    assert torch.equal(pool[pages - 1], pool[pages - 3])
+    table[0, 0] = pages - 3
+    pool[pages - 1].zero_()
+    got = b200attn.kv4_load(pool, table, None, 150)
+    for x, y in zip(got, (k, v)):
+        assert torch.equal(x.cpu().double(), values(y))
+    for t in (3, 40, 129):
+        q, ko = (torch.randn(1, heads, t, D, generator=g).bfloat16().to(cuda) for _ in range(2))
+        vo = torch.randn(1, t, heads, D, generator=g).bfloat16().to(cuda)
+        check(b200attn.kv4_joint_attention(q, ko, vo, pool, table, 150), q, ko, vo, values(k), values(v), [(150, t)])
+
+
+@pytest.mark.gpu
+def test_dense_attention_ignores_values_behind_the_valid_keys(cuda):
+    """The dense joint attention: infinities and NaN in K and V behind the valid keys of the
+    prefix and of the call do not reach the output."""
+    g = torch.Generator().manual_seed(9)
+    b, h, t, p = 2, 2, 200, 300
+    q, k = (torch.randn(b, h, t, D, generator=g).bfloat16() for _ in range(2))
+    v = torch.randn(b, t, h, D, generator=g).bfloat16()
+    pk, pv = (torch.randn(b, h, p, D, generator=g).bfloat16() for _ in range(2))
+    desc = [(300, 130), (37, 200)]
+    for i, (n, m) in enumerate(desc):
+        pk[i, :, n:], pv[i, :, n:] = math.nan, math.inf
+        k[i, :, m:], v[i, m:] = math.inf, math.nan
+    got = b200attn.joint_attention(*(x.to(cuda) for x in (q, k, v, pk, pv)),
+                                   desc=torch.tensor(desc, dtype=torch.int32, device=cuda))
+    check(got, q, k, v, pk.double(), pv.double(), desc)
+
+
+@pytest.mark.gpu
+def test_calls_at_once_on_two_streams(cuda):
+    """Two streams that attend over and extend the same pool at the same time, each with its
+    own sequences and workspace."""
+    pool, table, g = paged(cuda, [1200, 900], 4)
+    dense = torch.randn(2, 2, 4, 1200, D, generator=g).bfloat16()
+    b200attn.kv4_store(dense[0].to(cuda), dense[1].to(cuda), pool, table, count=i32(cuda, 1200, 900))
+    work = []
+    for i, t in ((0, 6), (1, 150)):
+        q, ko = (torch.randn(1, 4, t, D, generator=g).bfloat16().to(cuda) for _ in range(2))
+        vo = torch.randn(1, t, 4, D, generator=g).bfloat16().to(cuda)
+        work.append((torch.cuda.Stream(), q, ko, vo, table[i:i + 1].contiguous(), (1200, 900)[i], []))
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for s, q, ko, vo, tab, n, outs in work:
+            outs.append(b200attn.kv4_joint_attention(q, ko, vo, pool, tab, n, stream=s))
+    torch.cuda.synchronize()
+    for i, (s, q, ko, vo, tab, n, outs) in enumerate(work):
+        assert all(torch.equal(o, outs[0]) for o in outs)
+        check(outs[0], q, ko, vo, values(dense[0, i:i + 1]), values(dense[1, i:i + 1]), [(n, q.shape[2])])

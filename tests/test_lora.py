@@ -262,3 +262,39 @@ def test_every_sequence_with_its_own_adapter(cuda, fmt):
     model.set_adapters(None)
     with pytest.raises(ValueError, match="no adapters"):
         model.prefix_fill(embs, adapters=ids)
+
+
+@pytest.mark.gpu
+def test_rows_behind_32_bit_offsets(cuda):
+    """y of more than 2^32 elements: requests at its start and end."""
+    rows, n, k, rank = 350000, 12296, 64, 8
+    g = torch.Generator().manual_seed(2)
+    x = torch.randn(rows, k, device=cuda, dtype=torch.bfloat16)
+    y = torch.zeros(rows, n, device=cuda, dtype=torch.bfloat16)
+    a = (torch.randn(2, rank, k, generator=g) * k ** -0.5).bfloat16()
+    b = torch.randn(2, n, rank, generator=g).bfloat16()
+    seg = torch.tensor([0, 3, rows - 130, rows], dtype=torch.int32)
+    who = torch.tensor([1, -1, 0], dtype=torch.int32)
+    b200attn.lora_add(x, a.to(cuda), b.to(cuda), y, seg.to(cuda), who.to(cuda))
+    assert not y[3:rows - 130].any()
+    for r, e in ((slice(0, 3), 1), (slice(rows - 130, rows), 0)):
+        ident = torch.tensor([0, r.stop - r.start])
+        check(y[r], x[r].cpu(), torch.zeros(r.stop - r.start, n), a, b, None, ident, torch.tensor([e]))
+
+
+@pytest.mark.gpu
+def test_calls_at_once_on_two_streams(cuda):
+    g = torch.Generator().manual_seed(12)
+    args = []
+    for lens, k, n, rank in (([300, 5], 1024, 2048, 16), ([1000], 512, 768, 128)):
+        x, y, a, b, scale, seg, who = make(g, lens, [0] * len(lens), k, n, rank, 1)
+        args.append((torch.cuda.Stream(), [t.to(cuda) for t in (x, a, b, y, seg, who)], [], (x, y, a, b, None, seg, who)))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for s, dev, outs, _ in args:
+            with torch.cuda.stream(s):
+                outs.append(b200attn.lora_add(*dev, out=torch.empty_like(dev[3])))
+    torch.cuda.synchronize()
+    for s, dev, outs, (x, y, a, b, scale, seg, who) in args:
+        assert all(torch.equal(o, outs[0]) for o in outs)
+        check(outs[0], x, y, a, b, scale, seg, who)
