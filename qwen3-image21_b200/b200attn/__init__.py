@@ -589,6 +589,25 @@ def _expect(t, name: str, dtype, shape, device, dense: bool = True) -> None:
     raise ValueError(f"{name} must be contiguous")
 
 
+def _status_ptr(status, device) -> Optional[int]:
+    """The address of a status word, an int32 tensor on the device that computes."""
+    import torch
+    if status is None:
+        return None
+    if status.dtype is not torch.int32 or status.device != device or status.numel() < 1:
+        raise ValueError(f"status must be an int32 tensor on {device}")
+    return status.data_ptr()
+
+
+def _workspace(workspace, device) -> Tuple[Optional[int], int]:
+    """Address and bytes of a workspace on the device that computes."""
+    if workspace is None:
+        return None, 0
+    if workspace.device != device or not workspace.is_contiguous():
+        raise ValueError(f"workspace must be a contiguous tensor on {device}")
+    return workspace.data_ptr(), workspace.numel() * workspace.element_size()
+
+
 class _Launch:
     """Makes t's device current and, where a stream is given, that stream: the library
     launches on the current device, and what is allocated meanwhile belongs to the stream
@@ -651,7 +670,7 @@ def kv4_store(k, v, pool, page_table, start=None, count=None, status=None, strea
     ks, vs = ([s if n > 1 else 0 for s, n in zip(x.stride()[:3], x.shape)] for x in (k, v))
     with _Launch(pool, stream) as st:
         _check(lib().b200_kv4_store(ctypes.byref(view), _dptr(k), *ks, _dptr(v), *vs, b, h, t, d,
-                                    _dptr(start), _dptr(count), _dptr(status), st),
+                                    _dptr(start), _dptr(count), _status_ptr(status, pool.device), st),
                "b200_kv4_store")
 
 
@@ -671,7 +690,8 @@ def kv4_load(pool, page_table, lengths, max_len: int, k_out=None, v_out=None, st
         _expect(k_out, "k_out", torch.bfloat16, shape, pool.device)
         _expect(v_out, "v_out", torch.bfloat16, shape, pool.device)
         _check(lib().b200_kv4_load(ctypes.byref(view), _dptr(lengths), 1, _dptr(k_out),
-                                   _dptr(v_out), b, h, int(max_len), HEAD_DIM, _dptr(status), st),
+                                   _dptr(v_out), b, h, int(max_len), HEAD_DIM,
+                                   _status_ptr(status, pool.device), st),
                "b200_kv4_load")
     return k_out, v_out
 
@@ -704,11 +724,11 @@ def kv4_joint_attention(q_rot, k_rot, v, pool, page_table, prefix_len: int, desc
         if workspace is None and t > 64:  # up to there it needs none
             workspace = torch.empty(max(1, kv4_workspace_bytes(b, h, t, prefix_len)),
                                     dtype=torch.uint8, device=dev)
-        ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
+        ws, ws_bytes = _workspace(workspace, dev)
         _check(lib().b200_kv4_joint_attention(
             ctypes.byref(view), _dptr(q_rot), _dptr(k_rot), _dptr(v), b, h, t, int(prefix_len), d,
             _dptr(desc), _dptr(row_limit), float(d ** -0.5 if scale is None else scale), _dptr(out),
-            _dptr(workspace), ws_bytes, _dptr(status), st), "b200_kv4_joint_attention")
+            ws, ws_bytes, _status_ptr(status, dev), st), "b200_kv4_joint_attention")
     return out
 
 
@@ -753,8 +773,8 @@ def kv4_attention_forward(q, k, v, pool, page_table, prefix_len: int, norm_q_w, 
             _check(lib().b200_kv4_attn_workspace_bytes(ctypes.byref(args), ctypes.byref(n)),
                    "b200_kv4_attn_workspace_bytes")
             workspace = torch.empty(max(n.value, 1), dtype=torch.uint8, device=q.device)
-        args.workspace = workspace.data_ptr()
-        args.workspace_bytes = workspace.numel() * workspace.element_size()
+        args.workspace, args.workspace_bytes = _workspace(workspace, pool.device)
+        args.status = _status_ptr(status, pool.device)
         _check(lib().b200_kv4_attn_fwd(ctypes.byref(args), ctypes.byref(view), st),
                "b200_kv4_attn_fwd")
     return out
@@ -814,7 +834,8 @@ def lora_add(x, a, b, y, seg_start, seg_adapter, scale=None, out=None, status=No
     with _Launch(x, stream) as st:
         _check(lib().b200_lora_add(_dptr(x), strides[0], _dptr(a), _dptr(b), _dptr(y), strides[1],
                                    _dptr(out), strides[2], _dptr(seg_start), _dptr(seg_adapter),
-                                   _dptr(scale), rows, segments, e, n, k, rank, _dptr(status), st),
+                                   _dptr(scale), rows, segments, e, n, k, rank,
+                                   _status_ptr(status, dev), st),
                "b200_lora_add")
     return out
 

@@ -30,7 +30,8 @@ class AdapterBank:
         self.scale = torch.tensor(scales, dtype=torch.float32, device=device)
         self.linears: Dict[str, Tuple] = {}
         for name in sorted({n for a in adapters for n in a}):
-            if name.split(".", 2)[0] != "transformer_blocks" or name.split(".", 2)[2] not in TARGETS:
+            parts = name.split(".", 2)
+            if len(parts) != 3 or parts[0] != "transformer_blocks" or parts[2] not in TARGETS:
                 raise ValueError(f"{name} is not a block linear")
             pairs = [a.get(name) for a in adapters]
             shapes = {(p[0].shape[1], p[1].shape[0]) for p in pairs if p is not None}

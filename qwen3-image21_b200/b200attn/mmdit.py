@@ -588,6 +588,11 @@ class MMDiT:
     def set_adapters(self, bank) -> None:
         """The adapter bank (b200attn.lora.AdapterBank) whose adapters prefix_fill, step and
         denoise may name per sequence; None: none."""
+        if bank is not None:
+            shapes = weight_shapes(self.cfg)
+            for name, (a, b) in bank.linears.items():
+                if shapes.get(name + ".weight") != (b.shape[1], a.shape[2]):
+                    raise ValueError(f"{name}: {(b.shape[1], a.shape[2])} is not this model's shape")
         self.adapters = bank
 
     def _batch_adapters(self, ids, B: int, T: int):

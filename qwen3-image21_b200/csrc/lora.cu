@@ -42,6 +42,7 @@ constexpr int kMaxStages = 8;
 constexpr int kMaxC = 16;
 constexpr int kMaxExtent = 1 << 30;      // of K and N
 constexpr int kBarBytes = 512;
+constexpr int kMaxSmem = 227 * 1024;
 // Columns times groups of 4 rows of u up to which every CTA of a cluster adds the partials up
 // for itself, which saves one exchange between the CTAs.
 constexpr int kDirect = 256;
@@ -268,8 +269,8 @@ __global__ void __launch_bounds__(kLThreads, 2)
   if (adapter < 0) {  // the whole cluster: nothing to add (rows of y are copied to out)
     if (rows > 0 && p.out != p.y) {
       const int c0 = n_first * kTN, c1 = min((n_first + nb) * kTN, p.n);
-      const int per = (c1 - c0) / 8;
-      for (int i = threadIdx.x; i < rows * per; i += kLThreads) {
+      const int64_t per = (c1 - c0) / 8;
+      for (int64_t i = threadIdx.x; i < rows * per; i += kLThreads) {
         const int64_t r = row0 + i / per, c = c0 + (i % per) * 8;
         *reinterpret_cast<uint4*>(p.out + r * p.ldo + c) =
             *reinterpret_cast<const uint4*>(p.y + r * p.ldy + c);
@@ -599,8 +600,10 @@ int lora_map(CUtensorMap* map, const void* base, int dims, int64_t d0, int64_t d
              : B200_ERR_CUDA;
 }
 
-int lora_attributes(int smem) {
-  if (cudaFuncSetAttribute(lora_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) == cudaSuccess &&
+// The same values on every call: threads that launch at the same time do not disturb each
+// other.
+int lora_attributes() {
+  if (cudaFuncSetAttribute(lora_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem) == cudaSuccess &&
       cudaFuncSetAttribute(lora_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess)
     return B200_OK;
   cudaGetLastError();
@@ -689,7 +692,7 @@ extern "C" int b200_lora_add(const void* x, int64_t ldx, const void* a, const vo
   const int64_t expect = std::min<int64_t>(tiles, (rows + kTM - 1) / kTM + segments / 2);
   const int steps = std::max((k + kTK - 1) / kTK, (n + kTN - 1) / kTN);
   int rc;
-  if ((rc = lora_attributes(smem_of(regions == 1 ? 7 : 6))) != B200_OK) return rc;
+  if ((rc = lora_attributes()) != B200_OK) return rc;
   // The ring: 3 stages with two CTAs per SM, or (rank over 64) 4 with one; where one CTA per
   // SM holds all tiles in clusters as large, the rest of its shared memory too.
   p.stages = regions == 1 ? 3 : 4;

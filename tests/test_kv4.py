@@ -474,3 +474,37 @@ def test_calls_at_once_on_two_streams(cuda):
     for i, (s, q, ko, vo, tab, n, outs) in enumerate(work):
         assert all(torch.equal(o, outs[0]) for o in outs)
         check(outs[0], q, ko, vo, values(dense[0, i:i + 1]), values(dense[1, i:i + 1]), [(n, q.shape[2])])
+
+
+@pytest.mark.gpu
+def test_status_and_workspace_elsewhere_are_refused(cuda):
+    pool, table, g = paged(cuda, [64], 1)
+    q = torch.zeros(1, 1, 200, D, dtype=torch.bfloat16, device=cuda)
+    v = q.transpose(1, 2).contiguous()
+    with pytest.raises(ValueError, match="status"):
+        b200attn.kv4_joint_attention(q, q, v, pool, table, 64, status=torch.zeros(1, dtype=torch.int32))
+    with pytest.raises(ValueError, match="workspace"):
+        b200attn.kv4_joint_attention(q, q, v, pool, table, 64, workspace=torch.zeros(1 << 26, dtype=torch.uint8))
+    with pytest.raises(b200attn.B200Error):
+        b200attn.kv4_joint_attention(q, q, v, pool, table, 64,
+                                     workspace=torch.zeros(64, dtype=torch.uint8, device=cuda))
+    with pytest.raises(b200attn.B200Error):
+        b200attn.kv4_joint_attention(q, q, v, pool, table, 65)
+    with pytest.raises(ValueError, match="status"):
+        b200attn.kv4_load(pool, table, None, 64, status=torch.zeros(1, dtype=torch.int64, device=cuda))
+
+
+@pytest.mark.gpu
+def test_an_empty_pool_reads_as_zeros(cuda):
+    pool = torch.empty(0, 2, BLOCK, dtype=torch.uint8, device=cuda)
+    table = torch.zeros(1, 1, dtype=torch.int32, device=cuda)
+    status = torch.zeros(1, dtype=torch.int32, device=cuda)
+    k, v = b200attn.kv4_load(pool, table, None, 64, status=status)
+    assert not k.any() and not v.any() and status.item() == b200attn.KV4_STATUS_BAD_PAGE
+    q = torch.randn(1, 2, 3, D, device=cuda).bfloat16()
+    vo = torch.randn(1, 3, 2, D, device=cuda).bfloat16()
+    none = torch.zeros(1, 0, dtype=torch.int32, device=cuda)     # no table at all: own keys only
+    check(b200attn.kv4_joint_attention(q, q, vo, pool, none, 0), q, q, vo, k, v, [(0, 3)])
+    status.zero_()
+    b200attn.kv4_store(q, q, pool, none, status=status)
+    assert status.item() == b200attn.KV4_STATUS_BAD_PAGE

@@ -216,6 +216,8 @@ def test_bank_refuses_what_does_not_fit():
         AdapterBank([good], scales=[1.0, 2.0], device="cpu")
     with pytest.raises(ValueError, match="block linear"):
         AdapterBank([{"proj_out": (torch.zeros(4, 8), torch.zeros(8, 4))}], device="cpu")
+    with pytest.raises(ValueError, match="block linear"):
+        AdapterBank([{"transformer_blocks.0": (torch.zeros(4, 8), torch.zeros(8, 4))}], device="cpu")
     n = "transformer_blocks.0.attn.to_q"
     with pytest.raises(ValueError, match="fit together"):
         AdapterBank([{n: (torch.zeros(4, 8), torch.zeros(8, 5))}], device="cpu")
@@ -259,6 +261,10 @@ def test_every_sequence_with_its_own_adapter(cuda, fmt):
         assert rel <= 1.5e-2, (b, rel)
     with pytest.raises(ValueError, match="adapter ids"):
         model.prefix_fill(embs, adapters=[0])
+    for wrong in ({"transformer_blocks.2.attn.to_q": (torch.zeros(8, 256), torch.zeros(256, 8))},
+                  {"transformer_blocks.0.attn.to_q": (torch.zeros(8, 128), torch.zeros(256, 8))}):
+        with pytest.raises(ValueError, match="shape"):
+            model.set_adapters(AdapterBank([wrong], device=cuda))
     model.set_adapters(None)
     with pytest.raises(ValueError, match="no adapters"):
         model.prefix_fill(embs, adapters=ids)
@@ -298,3 +304,40 @@ def test_calls_at_once_on_two_streams(cuda):
     for s, dev, outs, (x, y, a, b, scale, seg, who) in args:
         assert all(torch.equal(o, outs[0]) for o in outs)
         check(outs[0], x, y, a, b, scale, seg, who)
+
+
+@pytest.mark.gpu
+def test_a_status_word_elsewhere_is_refused(cuda):
+    g = torch.Generator().manual_seed(1)
+    x, y, a, b, scale, seg, who = (t.to(cuda) for t in make(g, [4], [0], 64, 64, 8, 1))
+    for status in (torch.zeros(1, dtype=torch.int32), torch.zeros(1, dtype=torch.int64, device=cuda),
+                   torch.zeros(0, dtype=torch.int32, device=cuda)):
+        with pytest.raises(ValueError, match="status"):
+            b200attn.lora_add(x, a, b, y, seg, who, status=status)
+
+
+@pytest.mark.gpu
+def test_ranks_from_several_threads(cuda):
+    """Host threads that launch with different ranks (and so different shared memory)."""
+    import threading
+    g = torch.Generator().manual_seed(3)
+    jobs = [make(g, [200], [0], 256, 512, r, 1) for r in (16, 128, 64, 72)]
+    outs, failed = {}, []
+
+    def run(i):
+        try:
+            x, y, a, b, scale, seg, who = (t.to(cuda) for t in jobs[i])
+            for _ in range(50):
+                outs[i] = b200attn.lora_add(x, a, b, y, seg, who, scale=scale, out=torch.empty_like(y))
+        except Exception as e:  # reported by the test's own thread
+            failed.append(e)
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(len(jobs))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not failed
+    for i, (x, y, a, b, scale, seg, who) in enumerate(jobs):
+        check(outs[i], x, y, a, b, scale, seg, who)
