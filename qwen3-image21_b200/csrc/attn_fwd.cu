@@ -256,7 +256,8 @@ __device__ __forceinline__ float row_sum(const uint32_t (&r)[4][32]) {
 // ones have P = 0, but 0 * V is NaN where V holds an infinity or a NaN there.  A row is 128
 // bytes of each of the tile's two regions, whatever the swizzle.  At most one tile of each
 // segment has such rows.
-__device__ __noinline__ void clear_v_rows(uint8_t* tile, int first, int lane) {
+__device__ __forceinline__ void clear_v_rows(uint8_t* tile, int first, int lane) {
+#pragma unroll 1
   for (int i = first * 8 + lane; i < kBN * 8; i += 32) {
     *reinterpret_cast<uint4*>(tile + i * 16) = make_uint4(0, 0, 0, 0);
     *reinterpret_cast<uint4*>(tile + kRegionBytes + i * 16) = make_uint4(0, 0, 0, 0);
