@@ -269,11 +269,12 @@ __global__ void __launch_bounds__(kLThreads, 2)
   if (adapter < 0) {  // the whole cluster: nothing to add (rows of y are copied to out)
     if (rows > 0 && p.out != p.y) {
       const int c0 = n_first * kTN, c1 = min((n_first + nb) * kTN, p.n);
-      const int64_t per = (c1 - c0) / 8;
-      for (int64_t i = threadIdx.x; i < rows * per; i += kLThreads) {
-        const int64_t r = row0 + i / per, c = c0 + (i % per) * 8;
-        *reinterpret_cast<uint4*>(p.out + r * p.ldo + c) =
-            *reinterpret_cast<const uint4*>(p.y + r * p.ldy + c);
+      for (int r = warp; r < rows; r += kLThreads / 32) {
+        const __nv_bfloat16* from = p.y + static_cast<int64_t>(row0 + r) * p.ldy;
+        __nv_bfloat16* to = p.out + static_cast<int64_t>(row0 + r) * p.ldo;
+#pragma unroll 4
+        for (int c = c0 + lane * 8; c < c1; c += 256)
+          *reinterpret_cast<uint4*>(to + c) = *reinterpret_cast<const uint4*>(from + c);
       }
     }
     __syncthreads();
