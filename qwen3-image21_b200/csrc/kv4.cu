@@ -1,12 +1,16 @@
 // kv4.cu — the paged 4-bit prefix cache of include/b200_kv4.h: store, read back, page
-// copies, and attention of few query rows straight from the 4-bit pages.
+// copies, and attention straight from the 4-bit pages for up to 64 query rows (128 of few
+// heads); for more rows the pages are expanded for the attention of attn_fwd.cu.
 //
-//   kv4_store_kernel  one warp per 16 tokens of a page and head: group maxima by shuffles,
-//                     numbers packed in registers, 16-byte stores in the block's order.
-//   kv4_load_kernel   the inverse; s * n is exact in bf16.
-//   kv4_copy_kernel   16-byte copies of page pairs passed by value.
-//   kv4_attn_kernel   see there.
-// All four are bound by HBM (or, at a few pages, by their launch).
+//   kv4_store_kernel      one warp per 16 tokens of a page and head: group maxima by shuffles,
+//                         numbers packed in registers, 16-byte stores in the block's order.
+//                         4 x 4096 tokens of 32 heads: 60.6 us, 87 % of HBM's copy rate.
+//   kv4_load_kernel       the inverse; s * n is exact in bf16.  The same tokens: 55.0 us, 95 %.
+//   kv4_copy_kernel       16-byte copies of page pairs passed by value.  120 pages of 16
+//                         layers: 174 us, 6.5 TB/s.
+//   kv4_attn_kernel       up to 32 query rows, see there.
+//   kv4_attn_tile_kernel  up to 64 (or 128), see there.
+// The first three are bound by HBM (or, at a few pages, by their launch).
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -359,9 +363,11 @@ __global__ void __launch_bounds__(256) kv4_copy_kernel(const __grid_constant__ C
 // rows and 8 queries as the columns: the expanded cache is the A operand, which takes the
 // whole of a warp's lanes even for one query, is expanded once for all J query tiles, and
 // costs half the instructions of the form with queries as rows.  The kernel is bound by the
-// instructions that expand the numbers: per 16 keys a warp issues about 260, and 4 warps
-// schedulers at HBM rate have 400 slots.  (A tcgen05 tile would need the expanded values
-// written to shared memory again.)
+// instructions that expand the numbers: a warp issues about 300 per 16 keys, half of them on
+// the half-rate ALU pipe, and HBM rate would leave a scheduler 400 cycles for them.  With 16
+// warps per SM a page and head takes 0.28 us of an SM; HBM alone would take 0.21.  16 single
+// tokens over 1.3k to 10.6k keys, 32 heads: 97 us, 3.2 TB/s; one over 512 keys: 6 us.  (A
+// tcgen05 tile would need the expanded values written to shared memory again.)
 //   S^T = K Q^T   K's values s * n are exact in bf16;
 //   O^T = V^T P^T V's too, P is rounded to bf16 as in the dense path; P^T comes out of S^T
 //                 by two 8x8 transposes (movmatrix).
