@@ -8,7 +8,7 @@
 //   1. CTA c multiplies its part of K: x tiles [128 x 64] and A tiles [rank x 64] arrive by
 //      TMA, u_c accumulates in TMEM (tcgen05.mma M128 N=rank).
 //   2. The partial sums meet through distributed shared memory: CTA c adds the C partials of
-//      its 128 / C rows in rank order, scales, rounds to bf16, and fetches the other rows
+//      its share of the rows in rank order, scales, rounds to bf16, and fetches the other rows
 //      (of few rows, each CTA adds up all).
 //   3. CTA c walks its part of N in 64-column steps: B tiles and y tiles by TMA, u B^T in
 //      TMEM (two accumulators), the epilogue adds y in shared memory and writes whole
@@ -17,7 +17,7 @@
 // step 3 start while step 2 runs.
 //
 // 4 requests of 4096 rows, 4096 -> 12288, rank 64: 177 us, 5.3 TB/s; step 1 runs at 4.8 TB/s,
-// step 2 takes 5 us, step 3 runs at 6.3 TB/s.  16 ragged requests of 4600 rows in all: 43 us,
+// step 2 takes 5 us, step 3 runs at 6.3 TB/s.  16 ragged requests of 4600 rows in all: 37 us,
 // of which 15 go into set-up, first loads and step 2.  4 single rows: 12.5 us, all latency.
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -45,7 +45,7 @@ constexpr uint32_t kAccCol = 128;
 constexpr int kMaxStages = 8;
 constexpr int kMaxC = 16;
 constexpr int kMaxExtent = 1 << 30;      // of K and N
-constexpr int kBarBytes = 512;
+constexpr int kBarBytes = 768;
 constexpr int kMaxSmem = 227 * 1024;
 // Columns times groups of 4 rows of u up to which every CTA of a cluster adds the partials up
 // for itself, which saves one exchange between the CTAs.
@@ -61,7 +61,7 @@ struct LoraParams {
   int32_t rows, segments, adapters, n, k, rank;
   int32_t rp;            // rank rounded up to 16
   int32_t stages, stage_bytes;
-  int32_t C, log_c;      // CTAs of a cluster, a power of two
+  int32_t C;             // CTAs of a cluster
   int32_t* status;
 };
 
@@ -177,19 +177,20 @@ __device__ __forceinline__ int find_tile(const LoraParams& p, int tile, int lane
 
 // Rows [row, row + 4) of one column of u: the C partials, loaded together (a remote load takes
 // about half a microsecond) and added in rank order.
-template <int C>
-__device__ __forceinline__ float4 sum_partials(const uint32_t (&at)[C]) {
-  float4 v[C];
+template <int kMost>
+__device__ __forceinline__ float4 sum_partials(const uint32_t (&at)[kMost], int C) {
+  float4 v[kMost];
 #pragma unroll
-  for (int c = 0; c < C; ++c) v[c] = peer_ld_f32x4(at[c]);
+  for (int c = 0; c < kMost; ++c) v[c] = peer_ld_f32x4(at[c]);
   float4 sum = v[0];
 #pragma unroll
-  for (int c = 1; c < C; ++c) {
-    sum.x += v[c].x;
-    sum.y += v[c].y;
-    sum.z += v[c].z;
-    sum.w += v[c].w;
-  }
+  for (int c = 1; c < kMost; ++c)
+    if (c < C) {
+      sum.x += v[c].x;
+      sum.y += v[c].y;
+      sum.z += v[c].z;
+      sum.w += v[c].w;
+    }
   return sum;
 }
 
@@ -215,6 +216,9 @@ __global__ void __launch_bounds__(kLThreads, 2)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(u_full + 8);
   int* tile_word = reinterpret_cast<int*>(u_full + 9);  // [3]: rows, adapter, first row
   volatile int* abort_flag = tile_word + 3;
+  int* k_from = tile_word + 4;        // [C + 1]: first step of K of each CTA
+  int* quad_from = k_from + kMaxC + 1;   // [C + 1]: first group of 4 rows that each CTA adds up
+  int* quad_of = quad_from + kMaxC + 1;  // [32]: the CTA of each group
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int C = p.C;
@@ -238,6 +242,14 @@ __global__ void __launch_bounds__(kLThreads, 2)
     *abort_flag = 0;
     fence_barrier_init();
     fence_proxy_async();
+  }
+  const int nkb = (p.k + kTK - 1) / kTK, nnb = (p.n + kTN - 1) / kTN;  // steps (K, N <= 2^30: 16
+  if (threadIdx.x >= 128 && threadIdx.x <= 128 + C) {                  // times them fit 32 bits)
+    const int c = threadIdx.x - 128, q0 = kTM / 4 * c / C;
+    k_from[c] = nkb * c / C;
+    quad_from[c] = q0;
+    if (c < C)
+      for (int q = q0; q < kTM / 4 * (c + 1) / C; ++q) quad_of[q] = c;
   }
   if (warp == 2) {
     tmem_alloc(tmem_slot, kLTmemCols);
@@ -263,12 +275,9 @@ __global__ void __launch_bounds__(kLThreads, 2)
     adapter = -1;
   }
   // This CTA's part of K and of N (the same for every tile)
-  const int nkb = (p.k + kTK - 1) / kTK, nnb = (p.n + kTN - 1) / kTN;
-  // (K, N <= 2^30: 16 times their steps of 64 stay in 32 bits)
-  auto k_begin = [&](int c) { return (nkb * c) >> p.log_c; };
-  const int nk = k_begin(rank + 1) - k_begin(rank);
-  const int n_first = (nnb * rank) >> p.log_c;
-  const int nb = ((nnb * (rank + 1)) >> p.log_c) - n_first;
+  const int nk = k_from[rank + 1] - k_from[rank];
+  const int n_first = nnb * rank / C;
+  const int nb = nnb * (rank + 1) / C - n_first;
 
   if (adapter < 0) {  // the whole cluster: nothing to add (rows of y are copied to out)
     if (rows > 0 && p.out != p.y) {
@@ -294,7 +303,7 @@ __global__ void __launch_bounds__(kLThreads, 2)
   // per_stage columns in each.
   const int per_stage = p.stage_bytes / (kTM * 4);
   const int nx = C == 1 ? 0 : p.rp > per_stage ? 2 : 1;
-  const int steps0 = nkb >> p.log_c, stage0 = (steps0 + NS - nx) % NS;  // of a CTA with steps0
+  const int steps0 = nkb / C, stage0 = (steps0 + NS - nx) % NS;  // of a CTA with steps0
   auto part_at = [&](int steps, int col) {  // this CTA's address of a column of partials
     const int second = col >= per_stage ? 1 : 0;
     int st = stage0 + (steps - steps0) + second;  // steps is steps0 or one more
@@ -311,7 +320,7 @@ __global__ void __launch_bounds__(kLThreads, 2)
       tma_prefetch_desc(&tm_y);
       int it = 0;
       bool ok = true;
-      const int kb0 = k_begin(rank);
+      const int kb0 = k_from[rank];
       for (; it < nk; ++it) {
         const int s = it % NS;
         if (!mbar_wait(empty + s, ((it / NS) & 1) ^ 1, abort_flag)) {
@@ -454,9 +463,11 @@ __global__ void __launch_bounds__(kLThreads, 2)
               const int i = min(i0 + 128 * u, units - 1), col = i / quads, r = from + (i % quads) * 4;
               uint32_t at[CC];
 #pragma unroll
-              for (int c = 0; c < CC; ++c)
-                at[c] = peer_addr(part_at(k_begin(c + 1) - k_begin(c), col) + r, c);
-              sum[u] = sum_partials<CC>(at);
+              for (int c = 0; c < CC; ++c) {
+                const int from_c = c < C ? c : 0;  // past the last CTA: read, not added
+                at[c] = peer_addr(part_at(k_from[from_c + 1] - k_from[from_c], col) + r, from_c);
+              }
+              sum[u] = sum_partials<CC>(at, C);
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
@@ -471,18 +482,18 @@ __global__ void __launch_bounds__(kLThreads, 2)
           }
         };
         auto reduce_rows = [&](int from, int quads) {
-          if (C == 2) reduce(std::integral_constant<int, 2>(), from, quads);
-          else if (C == 4) reduce(std::integral_constant<int, 4>(), from, quads);
-          else if (C == 8) reduce(std::integral_constant<int, 8>(), from, quads);
+          if (C <= 2) reduce(std::integral_constant<int, 2>(), from, quads);
+          else if (C <= 4) reduce(std::integral_constant<int, 4>(), from, quads);
+          else if (C <= 8) reduce(std::integral_constant<int, 8>(), from, quads);
           else reduce(std::integral_constant<int, 16>(), from, quads);
         };
-        const int rs = kTM / C, quads = (rows + 3) / 4;
+        const int quads = (rows + 3) / 4;
         if (quads * p.rp <= kDirect) {  // few rows: every CTA adds them all up for itself
           reduce_rows(0, quads);
           epi_sync();
           if (e < C) peer_arrive(slice_ready, e);
         } else {                        // its own share, then the others' from them
-          reduce_rows(rank * rs, rs / 4);
+          reduce_rows(quad_from[rank] * 4, min(quad_from[rank + 1], quads) - quad_from[rank]);
           epi_sync();
           if (e < C) peer_arrive(slice_ready, e);
           ok = __all_sync(0xffffffffu, ok && wait_cluster(slice_ready, 0, abort_flag));
@@ -492,12 +503,12 @@ __global__ void __launch_bounds__(kLThreads, 2)
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
               const int i = min(i0 + 128 * u, all - 1), r = i / chunks;
-              v[u] = peer_ld_16b(peer_addr(u_chunk(r, i % chunks), r / rs));
+              v[u] = peer_ld_16b(peer_addr(u_chunk(r, i % chunks), quad_of[r / 4]));
             }
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
               const int i = i0 + 128 * u, r = i / chunks;
-              if (i < all && r / rs != rank) *reinterpret_cast<uint4*>(u_chunk(r, i % chunks)) = v[u];
+              if (i < all && quad_of[r / 4] != rank) *reinterpret_cast<uint4*>(u_chunk(r, i % chunks)) = v[u];
             }
           }
         }
@@ -692,7 +703,8 @@ extern "C" int b200_lora_add(const void* x, int64_t ldx, const void* a, const vo
   const auto smem_of = [&](int stages) { return stages * p.stage_bytes + regions * kXBytes + kBarBytes + 1024; };
   // Every request ends in a tile of its own: rows / 128 + segments tiles at most.  The
   // cluster is the largest whose tiles are expected to run all at once: with every request's
-  // last tile half full on average.
+  // last tile half full on average (16 ragged requests, 34 tiles: 72 us in clusters of 2, 43
+  // of 4, 37 of 6; of 8, 33 run at once and the 34th takes a second wave).
   const int64_t tiles = static_cast<int64_t>(rows) / kTM + std::min(segments, rows);
   const int64_t expect = std::min<int64_t>(tiles, (rows + kTM - 1) / kTM + segments / 2);
   const int steps = std::max((k + kTK - 1) / kTK, (n + kTN - 1) / kTN);
@@ -701,11 +713,8 @@ extern "C" int b200_lora_add(const void* x, int64_t ldx, const void* a, const vo
   // The ring: 3 stages with two CTAs per SM, or (rank over 64) 4 with one; where one CTA per
   // SM holds all tiles in clusters as large, the rest of its shared memory too.
   p.stages = regions == 1 ? 3 : 4;
-  p.C = 1;
-  while (p.C < kMaxC && 2 * p.C <= steps && expect <= active_clusters(2 * p.C, smem_of(p.stages))) {
-    p.C *= 2;
-    ++p.log_c;
-  }
+  p.C = std::min(kMaxC, steps);
+  while (p.C > 1 && expect > active_clusters(p.C, smem_of(p.stages))) --p.C;
   const int deep = regions == 1 ? 7 : 6;
   if (expect <= active_clusters(p.C, smem_of(deep))) p.stages = deep;
   const int C = p.C, smem = smem_of(p.stages);

@@ -101,6 +101,8 @@ CASES = [  # (rows of each request, adapters of them, K, N, rank, adapters)
     ([2, 2], [0, 1], 136, 64, 72, 2),
     ([2500, 2600, 17], [0, 1, 0], 256, 640, 48, 2),
     ([40000], [0], 64, 72, 64, 1),
+    *[([128] * tiles + [67], [i % 2 for i in range(tiles)] + [0], 1032, 1160, rank, 2)
+      for tiles, rank in ((4, 16), (7, 64), (12, 32), (18, 128), (26, 48), (40, 16), (57, 64), (100, 8))],
     ([20000, 1], [0, 1], 72, 64, 128, 2),
 ]
 
