@@ -98,7 +98,8 @@ int b200_kv4_attention_workspace_bytes(int32_t batch, int32_t heads, int32_t tar
  * knows, <= 64 * max_pages; prefix_valid is limited to it.  desc NULL: prefix_len and T.
  * What k_rot and v hold behind target_valid, and the cache behind prefix_valid, does not
  * reach the output, infinities and NaN included.  A row without any key gives NaN (the
- * reference's softmax of a row of -inf).
+ * reference's softmax of a row of -inf), and so does a row that sees a key whose score is NaN
+ * or +infinity (a stored group that was not finite reads as NaN).
  *
  * Few query rows run as one kernel straight from the 4-bit pages, without a workspace; for
  * more, the pages are expanded into the workspace once (b200_kv4_load's kernel) and the

@@ -139,9 +139,15 @@ __device__ __forceinline__ uint64_t f2add(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
-__device__ __forceinline__ float fmax3(float a, float b, float c) {
+// Maxima that are NaN where an operand is (fmaxf would drop it).
+__device__ __forceinline__ float fmax2_nan(float a, float b) {
   float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float fmax3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
 
@@ -149,7 +155,8 @@ __device__ __forceinline__ float fmax3(float a, float b, float c) {
 // the low mantissa bits of x + 1.5*2^23) and f in [-1/2, 1/2]; 2^f by a degree-4
 // polynomial with relative error < 3e-6 (coefficients from csrc/exp2_poly_fit.py); 2^j
 // applied by adding j to the exponent field.  x is clamped at -126.5 so j >= -126 (the
-// result is then at most ~1e-38 instead of 0, far below any row sum, which is >= 1).
+// result is then at most ~1e-38 instead of 0, far below any row sum, which is >= 1).  A NaN
+// does not come through it: softmax_row takes care of those by the row's maximum.
 constexpr float kExpC1 = 6.931241751e-01f;
 constexpr float kExpC2 = 2.402409911e-01f;
 constexpr float kExpC3 = 5.590642616e-02f;
@@ -182,7 +189,10 @@ constexpr int kPolyEvery = 4;
 // bf16 pairs, over S columns already read; the f32 p values stay in r for the row sum,
 // which the caller takes after handing P to the MMA warp (off the S -> P critical path).
 // Returns the factor the O accumulator must be scaled by (1 when m did not move).  A row
-// without any valid key so far keeps m = -inf and P = 0.
+// without any valid key so far keeps m = -inf and P = 0.  A row with a NaN or +inf among its
+// scores gets the factor NaN (and m = NaN), which makes its sum and so its output NaN
+// whatever later tiles hold: the maximum that carries the NaN costs nothing, and the exp2 of
+// the FMA pipe need not keep it.
 template <bool kMasked, bool kF16>
 __device__ __forceinline__ float softmax_row(uint32_t (&r)[4][32], const int valid,
                                              const float c, float& m, const uint32_t tS) {
@@ -199,17 +209,19 @@ __device__ __forceinline__ float softmax_row(uint32_t (&r)[4][32], const int val
   }
   float pm[8];
 #pragma unroll
-  for (int g = 0; g < 8; ++g) pm[g] = fmaxf(v(g * 16), v(g * 16 + 1));
+  for (int g = 0; g < 8; ++g) pm[g] = fmax2_nan(v(g * 16), v(g * 16 + 1));
 #pragma unroll
   for (int i = 1; i < 8; ++i)
 #pragma unroll
-    for (int g = 0; g < 8; ++g) pm[g] = fmax3(pm[g], v(g * 16 + 2 * i), v(g * 16 + 2 * i + 1));
+    for (int g = 0; g < 8; ++g) pm[g] = fmax3_nan(pm[g], v(g * 16 + 2 * i), v(g * 16 + 2 * i + 1));
   const float mx =
-      fmax3(fmax3(pm[0], pm[1], pm[2]), fmax3(pm[3], pm[4], pm[5]), fmaxf(pm[6], pm[7])) * c;
+      fmax3_nan(fmax3_nan(pm[0], pm[1], pm[2]), fmax3_nan(pm[3], pm[4], pm[5]),
+                fmax2_nan(pm[6], pm[7])) * c;
   float alpha = 1.f;
-  if (mx > m + kRescaleThreshold) {
-    alpha = ex2_approx(m - mx);  // 0 on the first tile (m = -inf)
-    m = mx;
+  if (!(mx <= m + kRescaleThreshold)) {  // NaN among them
+    const float to = mx + (mx - mx);     // +inf: NaN, as inf - inf is for the key itself
+    alpha = ex2_approx(m - to);          // 0 on the first tile (m = -inf)
+    m = to;
   }
   const uint64_t cc = f2pack(c, c);
   // A row that has not seen a valid key keeps m = -inf; its masked S (-inf) must give
