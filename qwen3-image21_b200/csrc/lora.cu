@@ -139,7 +139,24 @@ __device__ __forceinline__ uint32_t lora_pack(float lo, float hi) {
   return *reinterpret_cast<uint32_t*>(&v);
 }
 
+// The barrier of the four epilogue warps.  It has no limit, so every path of theirs passes the
+// same ones: whether a wait of theirs ran out decides about the work between, never about a
+// barrier.
 __device__ __forceinline__ void epi_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+
+// The same barrier; true if `ok` holds in all of its threads.
+__device__ __forceinline__ bool epi_all(bool ok) {
+  uint32_t all;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "bar.red.and.pred q, 1, 128, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(all)
+      : "r"(ok ? 1u : 0u)
+      : "memory");
+  return all != 0;
+}
 
 // The adapter and rows of tile `tile`; all lanes of one warp call it.  Returns the number of
 // rows, 0 when there is no such tile.
@@ -425,91 +442,91 @@ __global__ void __launch_bounds__(kLThreads, 2)
     };
     // 16-byte chunk j (8 of the rank) of row r in u_buf
     auto u_chunk = [&](int r, int j) { return u_buf + (j >> 3) * kXBytes + r * 128 + (((j & 7) ^ (r & 7)) << 4); };
-    if (ok) {
-      if (C == 1) {
-        for (int c = 0; c < p.rp && mine > 0; c += 16) {
-          uint32_t r[16];
-          u_cols(c, r);
+    if (C == 1) {
+      for (int c = 0; c < p.rp && mine > 0 && ok; c += 16) {
+        uint32_t r[16];
+        u_cols(c, r);
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            uint32_t w[4];
+        for (int j = 0; j < 2; ++j) {
+          uint32_t w[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              w[e] = lora_pack(__uint_as_float(r[8 * j + 2 * e]) * scale, __uint_as_float(r[8 * j + 2 * e + 1]) * scale);
-            *reinterpret_cast<uint4*>(u_chunk(tr, c / 8 + j)) = make_uint4(w[0], w[1], w[2], w[3]);
-          }
+          for (int e = 0; e < 4; ++e)
+            w[e] = lora_pack(__uint_as_float(r[8 * j + 2 * e]) * scale, __uint_as_float(r[8 * j + 2 * e + 1]) * scale);
+          *reinterpret_cast<uint4*>(u_chunk(tr, c / 8 + j)) = make_uint4(w[0], w[1], w[2], w[3]);
         }
-      } else {
-        for (int c = 0; c < p.rp && mine > 0; c += 16) {
-          uint32_t r[16];
-          u_cols(c, r);
+      }
+    } else {
+      for (int c = 0; c < p.rp && mine > 0 && ok; c += 16) {
+        uint32_t r[16];
+        u_cols(c, r);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) part_at(nk, c + i)[tr] = __uint_as_float(r[i]);
-        }
-        fence_proxy_async();  // the ring stages under the partials are TMA targets again later
-        epi_sync();
-        const int e = threadIdx.x - 128;
+        for (int i = 0; i < 16; ++i) part_at(nk, c + i)[tr] = __uint_as_float(r[i]);
+      }
+      fence_proxy_async();  // the ring stages under the partials are TMA targets again later
+      ok = epi_all(ok);
+      const int e = threadIdx.x - 128;
+      if (ok) {  // else the other CTAs' waits for this one's partials run out too
         if (e < C) peer_arrive(part_ready, e);
         ok = __all_sync(0xffffffffu, wait_cluster(part_ready, 0, abort_flag));
-        // Sums of `quads` groups of 4 rows from row `from` on, one column of one group at a
-        // time: U of them in flight.
-        auto reduce = [&](auto c_tag, int from, int quads) {
-          constexpr int CC = decltype(c_tag)::value, U = CC >= 8 ? 1 : 8 / CC;
-          const int units = p.rp * quads;
-          for (int i0 = e; ok && i0 < units; i0 += 128 * U) {
-            float4 sum[U];
+      }
+      // Sums of `quads` groups of 4 rows from row `from` on, one column of one group at a
+      // time: U of them in flight.
+      auto reduce = [&](auto c_tag, int from, int quads) {
+        constexpr int CC = decltype(c_tag)::value, U = CC >= 8 ? 1 : 8 / CC;
+        const int units = p.rp * quads;
+        for (int i0 = e; ok && i0 < units; i0 += 128 * U) {
+          float4 sum[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-              const int i = min(i0 + 128 * u, units - 1), col = i / quads, r = from + (i % quads) * 4;
-              uint32_t at[CC];
+          for (int u = 0; u < U; ++u) {
+            const int i = min(i0 + 128 * u, units - 1), col = i / quads, r = from + (i % quads) * 4;
+            uint32_t at[CC];
 #pragma unroll
-              for (int c = 0; c < CC; ++c) {
-                const int from_c = c < C ? c : 0;  // past the last CTA: read, not added
-                at[c] = peer_addr(part_at(k_from[from_c + 1] - k_from[from_c], col) + r, from_c);
-              }
-              sum[u] = sum_partials<CC>(at, C);
+            for (int c = 0; c < CC; ++c) {
+              const int from_c = c < C ? c : 0;  // past the last CTA: read, not added
+              at[c] = peer_addr(part_at(k_from[from_c + 1] - k_from[from_c], col) + r, from_c);
             }
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-              const int i = i0 + 128 * u, col = i / quads, r = from + (i % quads) * 4;
-              if (i >= units) break;
-              const float s4[4] = {sum[u].x, sum[u].y, sum[u].z, sum[u].w};
-#pragma unroll
-              for (int z = 0; z < 4; ++z)
-                reinterpret_cast<__nv_bfloat16*>(u_chunk(r + z, col >> 3))[col & 7] =
-                    __float2bfloat16_rn(s4[z] * scale);
-            }
+            sum[u] = sum_partials<CC>(at, C);
           }
-        };
-        auto reduce_rows = [&](int from, int quads) {
-          if (C <= 2) reduce(std::integral_constant<int, 2>(), from, quads);
-          else if (C <= 4) reduce(std::integral_constant<int, 4>(), from, quads);
-          else if (C <= 8) reduce(std::integral_constant<int, 8>(), from, quads);
-          else reduce(std::integral_constant<int, 16>(), from, quads);
-        };
-        const int quads = (rows + 3) / 4;
-        if (quads * p.rp <= kDirect) {  // few rows: every CTA adds them all up for itself
-          reduce_rows(0, quads);
-          epi_sync();
-          if (e < C) peer_arrive(slice_ready, e);
-        } else {                        // its own share, then the others' from them
-          reduce_rows(quad_from[rank] * 4, min(quad_from[rank + 1], quads) - quad_from[rank]);
-          epi_sync();
-          if (e < C) peer_arrive(slice_ready, e);
-          ok = __all_sync(0xffffffffu, ok && wait_cluster(slice_ready, 0, abort_flag));
-          const int chunks = p.rp / 8, all = rows * chunks;
-          for (int i0 = e; ok && i0 < all; i0 += 128 * 4) {
-            uint4 v[4];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-              const int i = min(i0 + 128 * u, all - 1), r = i / chunks;
-              v[u] = peer_ld_16b(peer_addr(u_chunk(r, i % chunks), quad_of[r / 4]));
-            }
+          for (int u = 0; u < U; ++u) {
+            const int i = i0 + 128 * u, col = i / quads, r = from + (i % quads) * 4;
+            if (i >= units) break;
+            const float s4[4] = {sum[u].x, sum[u].y, sum[u].z, sum[u].w};
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-              const int i = i0 + 128 * u, r = i / chunks;
-              if (i < all && quad_of[r / 4] != rank) *reinterpret_cast<uint4*>(u_chunk(r, i % chunks)) = v[u];
-            }
+            for (int z = 0; z < 4; ++z)
+              reinterpret_cast<__nv_bfloat16*>(u_chunk(r + z, col >> 3))[col & 7] =
+                  __float2bfloat16_rn(s4[z] * scale);
+          }
+        }
+      };
+      auto reduce_rows = [&](int from, int quads) {
+        if (C <= 2) reduce(std::integral_constant<int, 2>(), from, quads);
+        else if (C <= 4) reduce(std::integral_constant<int, 4>(), from, quads);
+        else if (C <= 8) reduce(std::integral_constant<int, 8>(), from, quads);
+        else reduce(std::integral_constant<int, 16>(), from, quads);
+      };
+      const int quads = (rows + 3) / 4;
+      if (quads * p.rp <= kDirect) {  // few rows: every CTA adds them all up for itself
+        reduce_rows(0, quads);
+        epi_sync();
+        if (e < C) peer_arrive(slice_ready, e);
+      } else {                        // its own share, then the others' from them
+        reduce_rows(quad_from[rank] * 4, min(quad_from[rank + 1], quads) - quad_from[rank]);
+        epi_sync();
+        if (e < C) peer_arrive(slice_ready, e);
+        ok = __all_sync(0xffffffffu, ok && wait_cluster(slice_ready, 0, abort_flag));
+        const int chunks = p.rp / 8, all = rows * chunks;
+        for (int i0 = e; ok && i0 < all; i0 += 128 * 4) {
+          uint4 v[4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const int i = min(i0 + 128 * u, all - 1), r = i / chunks;
+            v[u] = peer_ld_16b(peer_addr(u_chunk(r, i % chunks), quad_of[r / 4]));
+          }
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const int i = i0 + 128 * u, r = i / chunks;
+            if (i < all && quad_of[r / 4] != rank) *reinterpret_cast<uint4*>(u_chunk(r, i % chunks)) = v[u];
           }
         }
       }
