@@ -430,7 +430,8 @@ __global__ void __launch_bounds__(kLThreads, 2)
     bool ok = mbar_wait(u_full, 0, abort_flag);
     ok = __all_sync(0xffffffffu, ok);
     tc_fence_after();
-    // u, 16 columns at a time; a CTA without any part of K has zeros
+    // u, 16 columns at a time; a CTA without any part of K has zeros.  Columns from the rank on
+    // are made zeros below: A has zeros there, but an infinity in x makes them NaN.
     auto u_cols = [&](int c, uint32_t (&r)[16]) {
       if (nk > 0) {
         tmem_ld16(tmem_base + lane_off + c, r);
@@ -452,7 +453,8 @@ __global__ void __launch_bounds__(kLThreads, 2)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             w[e] = lora_pack(__uint_as_float(r[8 * j + 2 * e]) * scale, __uint_as_float(r[8 * j + 2 * e + 1]) * scale);
-          *reinterpret_cast<uint4*>(u_chunk(tr, c / 8 + j)) = make_uint4(w[0], w[1], w[2], w[3]);
+          *reinterpret_cast<uint4*>(u_chunk(tr, c / 8 + j)) =
+              c + 8 * j < p.rank ? make_uint4(w[0], w[1], w[2], w[3]) : make_uint4(0, 0, 0, 0);
         }
       }
     } else {
@@ -495,7 +497,7 @@ __global__ void __launch_bounds__(kLThreads, 2)
 #pragma unroll
             for (int z = 0; z < 4; ++z)
               reinterpret_cast<__nv_bfloat16*>(u_chunk(r + z, col >> 3))[col & 7] =
-                  __float2bfloat16_rn(s4[z] * scale);
+                  __float2bfloat16_rn(col < p.rank ? s4[z] * scale : 0.f);
           }
         }
       };
