@@ -16,8 +16,8 @@
  * numbers n in [-7, 7]; the value is s * n.
  *   top = max |x| of the group;  s = top / 7 cut to 5 significant bits
  *   n = sign(x) * floor(|x| / s + 1/2)   (|x| / s < 7.44)
- *   top < 2^-100: s = 0, n = 0.  top >= 2^126 or not finite: s = NaN, so that the whole
- *   group reads as NaN.
+ *   top < 2^-100: s = 0, n = 0.  top >= 2^126 or not finite: s = NaN and n = 0, so that the
+ *   whole group reads as NaN.
  * 5 bits of s times 3 bits of n: every value is exactly a bf16 number, so reading the cache
  * rounds nothing.
  *

@@ -96,14 +96,20 @@ __device__ __forceinline__ float group_step(float top) {
   return __uint_as_float(__float_as_uint(top * kSeventh) & 0xfff80000u);
 }
 
-// The factor that number4 takes for a step (0 for a step of 0 or NaN, whose numbers are 0).
+// The factor that number4 takes for a step above 0.
 // |x| / s differs from a half by 0 or by at least 1/496 (x has 8 significant bits, s has 5,
 // n at most 3): 1 + 2^-13 sends exact halves away from zero and moves no other value (below
 // 7.44) across one.
 __device__ __forceinline__ float number_scale(float step) {
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(step));
-  return step > 0.f ? r * (1.f + 0x1p-13f) : 0.f;
+  return r * (1.f + 0x1p-13f);
+}
+
+// The numbers of a group, or 0 (8 in each nibble) for all of them where its step is 0 or NaN:
+// taken by the step, not by a factor of 0, because infinity * 0 has no number.
+__device__ __forceinline__ uint32_t numbers_of(float step, uint32_t numbers) {
+  return step > 0.f ? numbers : 0x88888888u;
 }
 
 // n + 8 of the 4 values of two bf16 pairs as 4 nibbles in the low half: x * scale + 8 is
@@ -204,7 +210,8 @@ __global__ void __launch_bounds__(128, 6) kv4_store_kernel(const StoreParams p) 
         const uint4 x = kx[o][c + z];
         step[c + z] = group_step(z ? bf16_hi(both) : bf16_lo(both));
         const float f = number_scale(step[c + z]);
-        words[c + z] = prmt(number4(x.x, x.y, f), number4(x.z, x.w, f), 0x5410);
+        words[c + z] =
+            numbers_of(step[c + z], prmt(number4(x.x, x.y, f), number4(x.z, x.w, f), 0x5410));
       }
     }
     if (have(8 * o + g)) {
@@ -227,7 +234,8 @@ __global__ void __launch_bounds__(128, 6) kv4_store_kernel(const StoreParams p) 
       both = __vmaxu2(both, __shfl_xor_sync(0xffffffffu, both, 16));
       const float s0 = group_step(bf16_lo(both)), s1 = group_step(bf16_hi(both));
       vs[c] = prmt(__float_as_uint(s0), __float_as_uint(s1), 0x7632);
-      vw[c] = prmt(number4(x0.x, x0.y, number_scale(s0)), number4(x1.x, x1.y, number_scale(s1)), 0x5410);
+      vw[c] = prmt(numbers_of(s0, number4(x0.x, x0.y, number_scale(s0))),
+                   numbers_of(s1, number4(x1.x, x1.y, number_scale(s1))), 0x5410);
     }
     const bool h0 = have(8 * o + 2 * t), h1 = have(8 * o + 2 * t + 1);
     uint8_t* vd = block + kVOff + octet * kOctetBytes + lane * 16;
