@@ -10,7 +10,7 @@ pages to the front of the pool.
 from __future__ import annotations
 
 import heapq
-from typing import Dict, List, Sequence, Tuple
+from typing import Callable, Dict, List, Optional, Sequence, Tuple
 
 import b200attn
 from b200attn import KV4_BLOCK_BYTES, KV4_PAGE_TOKENS as PAGE
@@ -54,6 +54,12 @@ class PageTables:
             self._uses[p] = 1
         return got
 
+    def _give_back(self, pages: Sequence[int]) -> None:
+        for p in pages:
+            self._uses[p] -= 1
+            if self._uses[p] == 0:
+                heapq.heappush(self._free, p)
+
     def add(self, length: int) -> int:
         """A new sequence with room for `length` tokens; returns its id."""
         if length < 0:
@@ -72,10 +78,12 @@ class PageTables:
         self._pages[new], self._length[new] = list(pages), self._length[seq]
         return new
 
-    def extend(self, seqs: Sequence[int], counts: Sequence[int]) -> Copies:
+    def extend(self, seqs: Sequence[int], counts: Sequence[int],
+               move: Optional[Callable[[Copies], None]] = None) -> Copies:
         """Room for counts[i] more tokens behind sequence seqs[i] (each named once).  A last
         page that is not full and that another sequence holds too is replaced by a copy of
-        its own.  All or nothing."""
+        its own.  All or nothing; `move` is given the copies before anything changes, and if
+        it raises, nothing does."""
         if len(set(seqs)) != len(seqs) or len(seqs) != len(counts) or any(n < 0 for n in counts):
             raise ValueError("seqs must be distinct, with one count of at least 0 each")
         uses: Dict[int, int] = {}
@@ -90,40 +98,45 @@ class PageTables:
                     own = last
             plan.append((seq, n, own, -(-(length + n) // PAGE) - len(pages)))
         got = self._take(sum(more + (own is not None) for _, _, own, more in plan))
-        copies: Copies = []
+        fresh = iter(got)
+        copies = [(own, next(fresh)) for _, _, own, _ in plan if own is not None]
+        if move is not None:
+            try:
+                move(copies)
+            except BaseException:
+                self._give_back(got)
+                raise
+        into = iter(copies)
         for seq, n, own, more in plan:
             pages = self._pages[seq]
             if own is not None:
-                page = got.pop(0)
-                copies.append((own, page))
+                pages[-1] = next(into)[1]
                 self._uses[own] -= 1
-                pages[-1] = page
-            pages += got[:more]
-            del got[:more]
+            pages += [next(fresh) for _ in range(more)]
             self._length[seq] += n
         return copies
 
     def free(self, seq: int) -> None:
         """Forgets a sequence; pages that no other sequence holds are free again."""
-        for p in self._pages.pop(seq):
-            self._uses[p] -= 1
-            if self._uses[p] == 0:
-                heapq.heappush(self._free, p)
+        self._give_back(self._pages.pop(seq))
         del self._length[seq]
 
-    def compact(self) -> Copies:
+    def compact(self, move: Optional[Callable[[Copies], None]] = None) -> Copies:
         """Moves the live pages onto the first ids: afterwards page i is live exactly if i <
-        num_pages - free_pages."""
+        num_pages - free_pages.  `move` as in extend."""
         live = self.num_pages - len(self._free)
         holes = sorted(p for p in self._free if p < live)
         high = [p for p in range(live, self.num_pages) if self._uses[p]]
-        move = dict(zip(high, holes))
-        for src, dst in move.items():
+        to = dict(zip(high, holes))
+        copies = list(to.items())
+        if move is not None:
+            move(copies)
+        for src, dst in copies:
             self._uses[dst], self._uses[src] = self._uses[src], 0
         for seq, pages in self._pages.items():
-            self._pages[seq] = [move.get(p, p) for p in pages]
+            self._pages[seq] = [to.get(p, p) for p in pages]
         self._free = list(range(live, self.num_pages))
-        return list(move.items())
+        return copies
 
 
 class KV4Cache:
@@ -147,14 +160,25 @@ class KV4Cache:
 
     def add(self, lengths: Sequence[int]) -> List[int]:
         """New sequences of these lengths, to be filled with ``store`` (all or none)."""
+        lengths = [int(n) for n in lengths]
+        if any(n < 0 for n in lengths):
+            raise ValueError("a length must not be negative")
         if self.pages_for(lengths) > self.tables.free_pages:
             raise OutOfPages(f"{self.pages_for(lengths)} pages wanted, {self.tables.free_pages} free")
-        return [self.tables.add(int(n)) for n in lengths]
+        return [self.tables.add(n) for n in lengths]
 
     def fork(self, seqs: Sequence[int]) -> List[int]:
+        """A fork of each sequence (all or none)."""
+        for s in seqs:
+            self.tables.length(s)
         return [self.tables.fork(s) for s in seqs]
 
     def free(self, seqs: Sequence[int]) -> None:
+        """Forgets these sequences, each named once (all or none)."""
+        for s in seqs:
+            self.tables.length(s)
+        if len(set(seqs)) != len(seqs):
+            raise ValueError("a sequence is freed once")
         for s in seqs:
             self.tables.free(s)
 
@@ -164,14 +188,12 @@ class KV4Cache:
 
     def extend(self, seqs: Sequence[int], counts: Sequence[int]) -> None:
         """Room for more tokens, to be filled with ``store`` from the old lengths on."""
-        self._move(self.tables.extend(seqs, counts))
+        self.tables.extend(seqs, counts, self._move)
 
     def compact(self) -> int:
         """Moves the live pages to the front of the pool; returns how many pages were moved.
         Views taken before are stale."""
-        copies = self.tables.compact()
-        self._move(copies)
-        return len(copies)
+        return len(self.tables.compact(self._move))
 
     def view(self, seqs: Sequence[int]) -> "KV4View":
         """The page tables of a batch as they are now (stale after extend, free, compact)."""
