@@ -9,7 +9,9 @@ pages to the front of the pool.
 """
 from __future__ import annotations
 
+import functools
 import heapq
+import threading
 from typing import Callable, Dict, List, Optional, Sequence, Tuple
 
 import b200attn
@@ -22,14 +24,25 @@ class OutOfPages(RuntimeError):
     """The pool has too few free pages; nothing was changed."""
 
 
+def _locked(call):
+    """The method, holding the object's lock."""
+    @functools.wraps(call)
+    def held(self, *args, **kwargs):
+        with self.lock:
+            return call(self, *args, **kwargs)
+    return held
+
+
 class PageTables:
     """Which pages hold which sequence's tokens (host only; moves no data).  Calls that need
-    page contents moved return the copies, whose sources and destinations are disjoint."""
+    page contents moved return the copies, whose sources and destinations are disjoint.
+    Threads may share the tables: each call holds ``lock``."""
 
     def __init__(self, num_pages: int):
         if num_pages < 0:
             raise ValueError("num_pages must not be negative")
         self.num_pages = num_pages
+        self.lock = threading.RLock()
         self._free = list(range(num_pages))  # a heap
         self._uses = [0] * num_pages         # sequences that hold the page
         self._pages: Dict[int, List[int]] = {}
@@ -40,9 +53,11 @@ class PageTables:
     def free_pages(self) -> int:
         return len(self._free)
 
+    @_locked
     def pages(self, seq: int) -> List[int]:
         return list(self._pages[seq])
 
+    @_locked
     def length(self, seq: int) -> int:
         return self._length[seq]
 
@@ -60,6 +75,7 @@ class PageTables:
             if self._uses[p] == 0:
                 heapq.heappush(self._free, p)
 
+    @_locked
     def add(self, length: int) -> int:
         """A new sequence with room for `length` tokens; returns its id."""
         if length < 0:
@@ -69,6 +85,7 @@ class PageTables:
         self._pages[seq], self._length[seq] = pages, length
         return seq
 
+    @_locked
     def fork(self, seq: int) -> int:
         """A new sequence with the same tokens, on the same pages."""
         pages = self._pages[seq]
@@ -78,6 +95,7 @@ class PageTables:
         self._pages[new], self._length[new] = list(pages), self._length[seq]
         return new
 
+    @_locked
     def extend(self, seqs: Sequence[int], counts: Sequence[int],
                move: Optional[Callable[[Copies], None]] = None) -> Copies:
         """Room for counts[i] more tokens behind sequence seqs[i] (each named once).  A last
@@ -116,11 +134,13 @@ class PageTables:
             self._length[seq] += n
         return copies
 
+    @_locked
     def free(self, seq: int) -> None:
         """Forgets a sequence; pages that no other sequence holds are free again."""
         self._give_back(self._pages.pop(seq))
         del self._length[seq]
 
+    @_locked
     def compact(self, move: Optional[Callable[[Copies], None]] = None) -> Copies:
         """Moves the live pages onto the first ids: afterwards page i is live exactly if i <
         num_pages - free_pages.  `move` as in extend."""
@@ -141,12 +161,13 @@ class PageTables:
 
 class KV4Cache:
     """Pools of `layers` layers (uint8 [layers, num_pages, heads, 9216]) with the accounting
-    above.  Work is enqueued on the current stream of the pool's device."""
+    above.  Work is enqueued on the current stream of the pool's device. Threads may share a cache."""
 
     def __init__(self, layers: int, heads: int, num_pages: int, device="cuda"):
         import torch
         self.layers, self.heads = layers, heads
         self.tables = PageTables(num_pages)
+        self.lock = self.tables.lock
         self.pool = torch.empty((layers, num_pages, heads, KV4_BLOCK_BYTES), dtype=torch.uint8,
                                 device=device)
 
@@ -163,10 +184,12 @@ class KV4Cache:
         lengths = [int(n) for n in lengths]
         if any(n < 0 for n in lengths):
             raise ValueError("a length must not be negative")
-        if self.pages_for(lengths) > self.tables.free_pages:
-            raise OutOfPages(f"{self.pages_for(lengths)} pages wanted, {self.tables.free_pages} free")
-        return [self.tables.add(n) for n in lengths]
+        with self.lock:
+            if self.pages_for(lengths) > self.tables.free_pages:
+                raise OutOfPages(f"{self.pages_for(lengths)} pages wanted, {self.tables.free_pages} free")
+            return [self.tables.add(n) for n in lengths]
 
+    @_locked
     def fork(self, seqs: Sequence[int]) -> List[int]:
         """A fork of each sequence (all or none)."""
         for s in seqs:
@@ -175,12 +198,13 @@ class KV4Cache:
 
     def free(self, seqs: Sequence[int]) -> None:
         """Forgets these sequences, each named once (all or none)."""
-        for s in seqs:
-            self.tables.length(s)
-        if len(set(seqs)) != len(seqs):
-            raise ValueError("a sequence is freed once")
-        for s in seqs:
-            self.tables.free(s)
+        with self.lock:
+            for s in seqs:
+                self.tables.length(s)
+            if len(set(seqs)) != len(seqs):
+                raise ValueError("a sequence is freed once")
+            for s in seqs:
+                self.tables.free(s)
 
     def _move(self, copies: Copies) -> None:
         if copies:
@@ -188,12 +212,14 @@ class KV4Cache:
 
     def extend(self, seqs: Sequence[int], counts: Sequence[int]) -> None:
         """Room for more tokens, to be filled with ``store`` from the old lengths on."""
-        self.tables.extend(seqs, counts, self._move)
+        with self.lock:
+            self.tables.extend(seqs, counts, self._move)
 
     def compact(self) -> int:
         """Moves the live pages to the front of the pool; returns how many pages were moved.
         Views taken before are stale."""
-        return len(self.tables.compact(self._move))
+        with self.lock:
+            return len(self.tables.compact(self._move))
 
     def view(self, seqs: Sequence[int]) -> "KV4View":
         """The page tables of a batch as they are now (stale after extend, free, compact)."""
@@ -208,8 +234,9 @@ class KV4View:
     def __init__(self, cache: KV4Cache, seqs: List[int]):
         import torch
         self.cache, self.seqs = cache, seqs
-        self.lengths = [cache.tables.length(s) for s in seqs]
-        rows = [cache.tables.pages(s) for s in seqs]
+        with cache.lock:
+            self.lengths = [cache.tables.length(s) for s in seqs]
+            rows = [cache.tables.pages(s) for s in seqs]
         width = max([1] + [len(r) for r in rows])
         self.page_table = torch.tensor([r + [-1] * (width - len(r)) for r in rows], dtype=torch.int32,
                                        device=cache.pool.device).view(len(seqs), width)
