@@ -9,6 +9,7 @@ pages to the front of the pool.
 """
 from __future__ import annotations
 
+import contextlib
 import functools
 import heapq
 import threading
@@ -159,9 +160,36 @@ class PageTables:
         return copies
 
 
+class ReuseOrder:
+    """Orders the reuse of pages between streams.  Pages become free while work that reads
+    them may still be queued, and may be taken for another stream's work: ``released`` marks
+    a stream's queue where it gave pages back (or queued copies of pages), and ``before_taking``
+    makes a stream wait for all marks.  Streams are torch streams; `event` makes an event."""
+
+    def __init__(self, event):
+        self._event = event
+        self._marks: Dict[int, Tuple] = {}  # a stream's handle -> (stream, its latest mark)
+
+    def released(self, stream) -> None:
+        mark = self._event()
+        mark.record(stream)
+        self._marks[stream.cuda_stream] = (stream, mark)
+
+    def before_taking(self, stream) -> None:
+        for _, mark in self._marks.values():
+            stream.wait_event(mark)
+
+
 class KV4Cache:
     """Pools of `layers` layers (uint8 [layers, num_pages, heads, 9216]) with the accounting
-    above.  Work is enqueued on the current stream of the pool's device. Threads may share a cache."""
+    above.  Work is enqueued on the current stream of the pool's device.
+
+    Threads and streams may share a cache.  ``free`` may be called as soon as the last work
+    that reads the sequences is queued on the current stream (or the current stream waits for
+    it): pages are taken again, by ``add``, ``extend`` or ``compact`` on any stream, behind
+    that work.  New pages are filled on the stream that took them, or behind it; a stream that
+    reads, forks, extends or compacts what another one stored waits for that one first.  Calls
+    made while a graph is captured are not ordered: that is for whoever replays it."""
 
     def __init__(self, layers: int, heads: int, num_pages: int, device="cuda"):
         import torch
@@ -170,6 +198,26 @@ class KV4Cache:
         self.lock = self.tables.lock
         self.pool = torch.empty((layers, num_pages, heads, KV4_BLOCK_BYTES), dtype=torch.uint8,
                                 device=device)
+        self._order = ReuseOrder(torch.cuda.Event)
+
+    @contextlib.contextmanager
+    def _pages_move(self, takes: bool, releases: bool):
+        """Holds the lock around a change of the tables and what it queues; orders the current
+        stream behind others' use of free pages, and others behind this one's."""
+        import torch
+        with self.lock:
+            stream = None
+            if self.pool.is_cuda:
+                with torch.cuda.device(self.pool.device):
+                    if not torch.cuda.is_current_stream_capturing():
+                        stream = torch.cuda.current_stream()
+            if takes and stream is not None:
+                self._order.before_taking(stream)
+            try:
+                yield
+            finally:
+                if releases and stream is not None:
+                    self._order.released(stream)
 
     @staticmethod
     def pages_for(lengths: Sequence[int]) -> int:
@@ -184,7 +232,7 @@ class KV4Cache:
         lengths = [int(n) for n in lengths]
         if any(n < 0 for n in lengths):
             raise ValueError("a length must not be negative")
-        with self.lock:
+        with self._pages_move(takes=True, releases=False):
             if self.pages_for(lengths) > self.tables.free_pages:
                 raise OutOfPages(f"{self.pages_for(lengths)} pages wanted, {self.tables.free_pages} free")
             return [self.tables.add(n) for n in lengths]
@@ -198,7 +246,7 @@ class KV4Cache:
 
     def free(self, seqs: Sequence[int]) -> None:
         """Forgets these sequences, each named once (all or none)."""
-        with self.lock:
+        with self._pages_move(takes=False, releases=True):
             for s in seqs:
                 self.tables.length(s)
             if len(set(seqs)) != len(seqs):
@@ -212,13 +260,13 @@ class KV4Cache:
 
     def extend(self, seqs: Sequence[int], counts: Sequence[int]) -> None:
         """Room for more tokens, to be filled with ``store`` from the old lengths on."""
-        with self.lock:
+        with self._pages_move(takes=True, releases=True):
             self.tables.extend(seqs, counts, self._move)
 
     def compact(self) -> int:
         """Moves the live pages to the front of the pool; returns how many pages were moved.
         Views taken before are stale."""
-        with self.lock:
+        with self._pages_move(takes=True, releases=True):
             return len(self.tables.compact(self._move))
 
     def view(self, seqs: Sequence[int]) -> "KV4View":
