@@ -644,27 +644,29 @@ class MMDiT:
             emb[b, :lengths[b]] = e.to(self.device, torch.bfloat16)
         x = self.text_embed(emb.view(B * P, cfg.text_dim)).contiguous()
         shape = (B, cfg.heads, P, HEAD_DIM)
-        if kv4 is not None:
-            cache = kv4.view(kv4.add(lengths))
-        else:
-            if offload:
-                alloc = lambda: torch.empty(shape, dtype=torch.bfloat16).pin_memory()
-            else:
-                alloc = lambda: torch.zeros(shape, dtype=torch.bfloat16, device=self.device)
-            cache = PrefixCache(k=[alloc() for _ in range(cfg.layers)],
-                                v=[alloc() for _ in range(cfg.layers)], lengths=lengths)
-        lay = b200attn.joint_layout(P, None, [], (0, 0))
-        pe = torch.from_numpy(b200attn.rope_pe(lay["img_shapes"], lay["image_pad_mask"], AXES,
-                                               ROPE_THETA)[:P]).to(self.device)
-        limits = torch.from_numpy(b200attn.block_causal_limits(lay["image_ids"][:P])).to(self.device)
-        desc = torch.tensor([[0, n] for n in lengths], dtype=torch.int32, device=self.device)
-        mod = self.modulation(self.zero_time_embed())
+        seqs: List[int] = []
         try:
+            if kv4 is not None:
+                seqs = kv4.add(lengths)
+                cache = kv4.view(seqs)
+            else:
+                if offload:
+                    alloc = lambda: torch.empty(shape, dtype=torch.bfloat16).pin_memory()
+                else:
+                    alloc = lambda: torch.zeros(shape, dtype=torch.bfloat16, device=self.device)
+                cache = PrefixCache(k=[alloc() for _ in range(cfg.layers)],
+                                    v=[alloc() for _ in range(cfg.layers)], lengths=lengths)
+            lay = b200attn.joint_layout(P, None, [], (0, 0))
+            pe = torch.from_numpy(b200attn.rope_pe(lay["img_shapes"], lay["image_pad_mask"], AXES,
+                                                   ROPE_THETA)[:P]).to(self.device)
+            limits = torch.from_numpy(b200attn.block_causal_limits(lay["image_ids"][:P])).to(self.device)
+            desc = torch.tensor([[0, n] for n in lengths], dtype=torch.int32, device=self.device)
+            mod = self.modulation(self.zero_time_embed())
             self._run_blocks(x, B, P, mod, pe, None, desc, row_limit=limits, kv_out=cache,
                              adapters=adapters)
         except BaseException:
-            if kv4 is not None:
-                kv4.free(cache.seqs)
+            if seqs:
+                kv4.free(seqs)
             raise
         return cache
 
@@ -726,23 +728,28 @@ def denoise(model: MMDiT, pos_embs: Sequence, neg_embs: Optional[Sequence], grid
     ids = adapters
     if adapters is not None and neg_embs is not None:
         ids = [a for a in adapters for _ in range(2)]
-    seqs: List[int] = []
-    if kv4 is not None and kv4 is not False:
-        from b200attn.kv4 import KV4Cache
-        keys = [(id(e), None if ids is None else ids[i]) for i, e in enumerate(embs)]
-        first = [keys.index(k) for k in keys]
-        once = sorted(set(first))
-        if kv4 is True:
-            kv4 = KV4Cache(model.cfg.layers, model.cfg.heads,
-                           KV4Cache.pages_for([int(embs[i].shape[0]) for i in once]), model.device)
-        filled = model.prefix_fill([embs[i] for i in once], kv4=kv4,
-                                   adapters=None if ids is None else [ids[i] for i in once])
-        own = dict(zip(once, filled.seqs))
-        seqs = [own[i] if i == f else kv4.fork([own[f]])[0] for i, f in enumerate(first)]
-        cache = kv4.view(seqs)
-    else:
-        cache = model.prefix_fill(embs, offload=offload_cache, adapters=ids)
+    seqs: List[int] = []  # of a 4-bit cache, to be freed at the end
     try:
+        if kv4 is not None and kv4 is not False:
+            from b200attn.kv4 import KV4Cache
+            keys = [(id(e), None if ids is None else ids[i]) for i, e in enumerate(embs)]
+            first = [keys.index(k) for k in keys]
+            once = sorted(set(first))
+            if kv4 is True:
+                kv4 = KV4Cache(model.cfg.layers, model.cfg.heads,
+                               KV4Cache.pages_for([int(embs[i].shape[0]) for i in once]), model.device)
+            filled = model.prefix_fill([embs[i] for i in once], kv4=kv4,
+                                       adapters=None if ids is None else [ids[i] for i in once])
+            seqs += filled.seqs
+            own = dict(zip(once, filled.seqs))
+            rows = []
+            for i, f in enumerate(first):
+                if i != f:
+                    seqs += kv4.fork([own[f]])
+                rows.append(own[i] if i == f else seqs[-1])
+            cache = kv4.view(rows)
+        else:
+            cache = model.prefix_fill(embs, offload=offload_cache, adapters=ids)
         pe = model.target_pe(cache.lengths, grid)
         desc = cached_desc(cache, T, model.device)
         sigmas = flow_match_sigmas(steps, T)
