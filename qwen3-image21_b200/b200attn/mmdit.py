@@ -715,7 +715,7 @@ def denoise(model: MMDiT, pos_embs: Sequence, neg_embs: Optional[Sequence], grid
     with true CFG (neg + scale * (pos - neg)) when neg_embs is given.  Latents stay f32;
     the transformer reads them as bf16.  offload_cache keeps the prefix cache in pinned host
     memory (set_kv_cache_offload).  kv4 (a b200attn.kv4.KV4Cache, True: one made to fit)
-    keeps it in 4 bits; prompts that are given as one and the same tensor, like a negative
+    keeps it in 4 bits on the GPU (not with offload_cache); prompts that are given as one and the same tensor, like a negative
     prompt for every request, are then computed once and share their pages, which are free
     again at the end.  adapters: the adapter id of each prompt (its negative takes the same),
     or None.  Returns the final packed latents f32 [n, T, C]."""
@@ -738,7 +738,7 @@ def denoise(model: MMDiT, pos_embs: Sequence, neg_embs: Optional[Sequence], grid
             if kv4 is True:
                 kv4 = KV4Cache(model.cfg.layers, model.cfg.heads,
                                KV4Cache.pages_for([int(embs[i].shape[0]) for i in once]), model.device)
-            filled = model.prefix_fill([embs[i] for i in once], kv4=kv4,
+            filled = model.prefix_fill([embs[i] for i in once], offload=offload_cache, kv4=kv4,
                                        adapters=None if ids is None else [ids[i] for i in once])
             seqs += filled.seqs
             own = dict(zip(once, filled.seqs))
