@@ -596,13 +596,13 @@ class MMDiT:
         self.adapters = bank
 
     def _batch_adapters(self, ids, B: int, T: int):
+        if ids is not None and len(ids) != B:
+            raise ValueError(f"{len(ids)} adapter ids for {B} sequences")
         if ids is None or all(i is None or i < 0 for i in ids):
             return None
         from b200attn.lora import BatchAdapters
         if self.adapters is None:
             raise ValueError("the model has no adapters (set_adapters)")
-        if len(ids) != B:
-            raise ValueError(f"{len(ids)} adapter ids for {B} sequences")
         return BatchAdapters(self.adapters, ids, T)
 
     # -- prefix fill ---------------------------------------------------------------
@@ -725,6 +725,8 @@ def denoise(model: MMDiT, pos_embs: Sequence, neg_embs: Optional[Sequence], grid
     embs = list(pos_embs)
     if neg_embs is not None:  # sequence order: p0 pos, p0 neg, p1 pos, p1 neg, ...
         embs = [e for pair in zip(pos_embs, neg_embs) for e in pair]
+    if adapters is not None and len(adapters) != len(pos_embs):
+        raise ValueError(f"{len(adapters)} adapter ids for {len(pos_embs)} prompts")
     ids = adapters
     if adapters is not None and neg_embs is not None:
         ids = [a for a in adapters for _ in range(2)]
