@@ -589,6 +589,15 @@ def _expect(t, name: str, dtype, shape, device, dense: bool = True) -> None:
     raise ValueError(f"{name} must be contiguous")
 
 
+def _i32(n, name: str) -> int:
+    """n as an int; ValueError if it does not fit the library's 32 bits (ctypes would cut it
+    off without a word)."""
+    n = int(n)
+    if not -2 ** 31 <= n < 2 ** 31:
+        raise ValueError(f"{name} = {n} does not fit 32 bits")
+    return n
+
+
 def _status_ptr(status, device) -> Optional[int]:
     """The address of a status word, an int32 tensor on the device that computes."""
     import torch
@@ -679,9 +688,9 @@ def kv4_load(pool, page_table, lengths, max_len: int, k_out=None, v_out=None, st
     """Reads the cache back: (k, v) bf16 [B, H, max_len, 128], the dense prefix layout; rows
     from lengths[b] (int32 [B], or None: max_len) on are zeros."""
     import torch
-    h, b = pool.shape[1], page_table.shape[0]
+    h, b, max_len = pool.shape[1], page_table.shape[0], _i32(max_len, "max_len")
     view = _kv4_view(pool, page_table, b, h)
-    shape = (b, h, int(max_len), HEAD_DIM)
+    shape = (b, h, max_len, HEAD_DIM)
     if lengths is not None:
         _expect(lengths, "lengths", torch.int32, (b,), pool.device)
     with _Launch(pool, stream) as st:
@@ -690,7 +699,7 @@ def kv4_load(pool, page_table, lengths, max_len: int, k_out=None, v_out=None, st
         _expect(k_out, "k_out", torch.bfloat16, shape, pool.device)
         _expect(v_out, "v_out", torch.bfloat16, shape, pool.device)
         _check(lib().b200_kv4_load(ctypes.byref(view), _dptr(lengths), 1, _dptr(k_out),
-                                   _dptr(v_out), b, h, int(max_len), HEAD_DIM,
+                                   _dptr(v_out), b, h, max_len, HEAD_DIM,
                                    _status_ptr(status, pool.device), st),
                "b200_kv4_load")
     return k_out, v_out
@@ -706,6 +715,7 @@ def kv4_joint_attention(q_rot, k_rot, v, pool, page_table, prefix_len: int, desc
     [0, row_limit[i]).  workspace uint8 (kv4_workspace_bytes; allocated here when None)."""
     import torch
     b, h, t, d = q_rot.shape
+    prefix_len = _i32(prefix_len, "prefix_len")
     dev = pool.device
     bf = torch.bfloat16
     _expect(q_rot, "q_rot", bf, (b, h, t, d), dev)
@@ -726,7 +736,7 @@ def kv4_joint_attention(q_rot, k_rot, v, pool, page_table, prefix_len: int, desc
                                     dtype=torch.uint8, device=dev)
         ws, ws_bytes = _workspace(workspace, dev)
         _check(lib().b200_kv4_joint_attention(
-            ctypes.byref(view), _dptr(q_rot), _dptr(k_rot), _dptr(v), b, h, t, int(prefix_len), d,
+            ctypes.byref(view), _dptr(q_rot), _dptr(k_rot), _dptr(v), b, h, t, prefix_len, d,
             _dptr(desc), _dptr(row_limit), float(d ** -0.5 if scale is None else scale), _dptr(out),
             ws, ws_bytes, _status_ptr(status, dev), st), "b200_kv4_joint_attention")
     return out
@@ -734,9 +744,10 @@ def kv4_joint_attention(q_rot, k_rot, v, pool, page_table, prefix_len: int, desc
 
 def kv4_workspace_bytes(batch: int, heads: int, target_len: int, prefix_len: int) -> int:
     """Scratch bytes of kv4_joint_attention for these sizes."""
+    sizes = [_i32(x, name) for x, name in ((batch, "batch"), (heads, "heads"), (target_len, "target_len"),
+                                           (prefix_len, "prefix_len"))]
     n = ctypes.c_size_t()
-    _check(lib().b200_kv4_attention_workspace_bytes(batch, heads, target_len, int(prefix_len),
-                                                    ctypes.byref(n)),
+    _check(lib().b200_kv4_attention_workspace_bytes(*sizes, ctypes.byref(n)),
            "b200_kv4_attention_workspace_bytes")
     return n.value
 
@@ -748,6 +759,7 @@ def kv4_attention_forward(q, k, v, pool, page_table, prefix_len: int, norm_q_w, 
     q, k, v bf16 [B,T,H,D] raw projections, Q/K RMSNorm + RoPE, then joint attention."""
     import torch
     b, t, h, d = q.shape
+    prefix_len = _i32(prefix_len, "prefix_len")
     for x, name in ((q, "q"), (k, "k"), (v, "v")):
         _expect(x, name, torch.bfloat16, (b, t, h, d), pool.device)
     for x, name in ((k_rot_out, "k_rot_out"), (v_out, "v_out")):
@@ -767,7 +779,7 @@ def kv4_attention_forward(q, k, v, pool, page_table, prefix_len: int, norm_q_w, 
         _expect(out, "out", torch.bfloat16, (b, t, h * d), pool.device)
         args = make_args(q, k, v, None, None, norm_q_w, norm_k_w, pe, out, desc, scale, eps,
                          k_rot_out, v_out, None, status, row_limit)
-        args.prefix_len = int(prefix_len)
+        args.prefix_len = prefix_len
         if workspace is None:
             n = ctypes.c_size_t()
             _check(lib().b200_kv4_attn_workspace_bytes(ctypes.byref(args), ctypes.byref(n)),
@@ -793,7 +805,7 @@ def kv4_copy_pages(pool, src: Sequence[int], dst: Sequence[int], stream=None):
     n = len(src)
     if n != len(dst):
         raise ValueError("src and dst must have the same length")
-    s, d = (ctypes.c_int32 * n)(*src), (ctypes.c_int32 * n)(*dst)
+    s, d = ((ctypes.c_int32 * n)(*(_i32(p, "a page") for p in x)) for x in (src, dst))
     with _Launch(pool, stream) as st:
         _check(lib().b200_kv4_copy_pages(_dptr(pool), layers, pages * heads * KV4_BLOCK_BYTES, pages,
                                          heads, s, d, n, st), "b200_kv4_copy_pages")
@@ -834,7 +846,7 @@ def lora_add(x, a, b, y, seg_start, seg_adapter, scale=None, out=None, status=No
     with _Launch(x, stream) as st:
         _check(lib().b200_lora_add(_dptr(x), strides[0], _dptr(a), _dptr(b), _dptr(y), strides[1],
                                    _dptr(out), strides[2], _dptr(seg_start), _dptr(seg_adapter),
-                                   _dptr(scale), rows, segments, e, n, k, rank,
+                                   _dptr(scale), _i32(rows, "rows"), segments, e, n, k, rank,
                                    _status_ptr(status, dev), st),
                "b200_lora_add")
     return out
