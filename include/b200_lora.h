@@ -31,8 +31,9 @@ extern "C" {
 /*
  *   x    device bf16 [rows, k], row stride ldx      a  device bf16 [adapters, rank, k]
  *   y    device bf16 [rows, n], row stride ldy      b  device bf16 [adapters, n, rank]
- *   out  device bf16 [rows, n], row stride ldo; out == y (with ldo == ldy) adds in place;
- *        otherwise out overlaps neither y nor x
+ *   out  device bf16 [rows, n], row stride ldo; out == y (with ldo == ldy) adds in place.
+ *        Otherwise out overlaps y in no element, and in either case a row of out no other row
+ *        of x (B200_ERR_INVALID); columns of one buffer that keep apart are no overlap
  *   seg_start   device int32 [segments + 1], non-decreasing: request s has the rows
  *               [seg_start[s], seg_start[s + 1]); limited to [0, rows]
  *   seg_adapter device int32 [segments]: the request's adapter, negative for none (its rows

@@ -680,6 +680,25 @@ int active_clusters(int C, int smem) {
 
 bool lora_al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// Whether writing `out` (rows of n, ldo apart) can disturb reads of `in` (rows of cols, ldi
+// apart) that are still to come.  Column ranges of one buffer that keep apart do not.  With
+// same_row, a row's own writes may hit its own reads: the whole cluster has read its rows of x
+// before any of it writes.
+bool lora_disturbs(const void* out, int64_t ldo, int64_t n, const void* in, int64_t ldi, int64_t cols,
+                   int64_t rows, bool same_row) {
+  using wide = __int128;
+  const wide o = reinterpret_cast<uintptr_t>(out) / 2, i = reinterpret_cast<uintptr_t>(in) / 2;
+  if (o + wide(rows - 1) * ldo + n <= i || i + wide(rows - 1) * ldi + cols <= o) return false;
+  if (rows == 1) return !same_row;
+  if (ldo != ldi) return true;
+  // row r of out starts m elements behind the start of row r + q of in
+  const wide d = o - i;
+  const wide q = d >= 0 ? d / ldi : -((-d + ldi - 1) / ldi);
+  const wide m = d - q * ldi;
+  const bool meets = m < cols, meets_next = m + n > ldi;  // row r + q, row r + q + 1
+  return same_row ? (meets && q != 0) || (meets_next && q != -1) : meets || meets_next;
+}
+
 }  // namespace
 }  // namespace b200
 
@@ -701,6 +720,8 @@ extern "C" int b200_lora_add(const void* x, int64_t ldx, const void* a, const vo
     if (!lora_al16(ptr)) return B200_ERR_INVALID;
   if (ldx < k || ldy < n || ldo < n || ldx % 8 != 0 || ldy % 8 != 0 || ldo % 8 != 0) return B200_ERR_INVALID;
   if (out == y && ldo != ldy) return B200_ERR_INVALID;
+  if (out != y && lora_disturbs(out, ldo, n, y, ldy, n, rows, false)) return B200_ERR_INVALID;
+  if (lora_disturbs(out, ldo, n, x, ldx, k, rows, true)) return B200_ERR_INVALID;
   LoraParams p{};
   p.y = static_cast<const __nv_bfloat16*>(y);
   p.out = static_cast<__nv_bfloat16*>(out);
