@@ -14,6 +14,7 @@ Names mirror the reference's functions on this path:
 """
 from __future__ import annotations
 
+import array
 import ctypes
 import os
 from typing import Optional, Sequence, Tuple
@@ -805,10 +806,14 @@ def kv4_copy_pages(pool, src: Sequence[int], dst: Sequence[int], stream=None):
     n = len(src)
     if n != len(dst):
         raise ValueError("src and dst must have the same length")
-    s, d = ((ctypes.c_int32 * n)(*(_i32(p, "a page") for p in x)) for x in (src, dst))
+    try:
+        s, d = array.array("i", src), array.array("i", dst)
+    except OverflowError:
+        raise ValueError("a page id does not fit 32 bits") from None
     with _Launch(pool, stream) as st:
         _check(lib().b200_kv4_copy_pages(_dptr(pool), layers, pages * heads * KV4_BLOCK_BYTES, pages,
-                                         heads, s, d, n, st), "b200_kv4_copy_pages")
+                                         heads, s.buffer_info()[0], d.buffer_info()[0], n, st),
+               "b200_kv4_copy_pages")
 
 
 # ----------------------------------------------------------------- per-request adapters
