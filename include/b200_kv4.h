@@ -99,7 +99,9 @@ int b200_kv4_attention_workspace_bytes(int32_t batch, int32_t heads, int32_t tar
  * What k_rot and v hold behind target_valid, and the cache behind prefix_valid, does not
  * reach the output, infinities and NaN included.  A row without any key gives NaN (the
  * reference's softmax of a row of -inf), and so does a row that sees a key whose score is NaN
- * or +infinity (a stored group that was not finite reads as NaN).
+ * or +infinity (a stored group that was not finite reads as NaN).  An infinity or NaN in v of
+ * a key that is valid but behind a row's row_limit may reach that row (0 * NaN is NaN, as in
+ * a softmax times V).
  *
  * Few query rows run as one kernel straight from the 4-bit pages, without a workspace; for
  * more, the pages are expanded into the workspace once (b200_kv4_load's kernel) and the

@@ -294,7 +294,9 @@ class KV4View:
         return self.cache.pool[layer]
 
     def store(self, layer: int, k, v, start=None, count=None) -> None:
-        """k, v bf16 [B, H, T, 128] into this layer's pages (see b200attn.kv4_store)."""
+        """k, v bf16 [B, H, T, 128] into this layer's pages (see b200attn.kv4_store).  Pages
+        that forks share are read by all of them: new tokens of a fork go behind its length
+        of before ``extend``, whose copy makes that page its own."""
         b200attn.kv4_store(k, v, self.pool(layer), self.page_table, start=start, count=count)
 
     def load(self, layer: int, lengths=None):

@@ -370,15 +370,20 @@ __global__ void __launch_bounds__(256) kv4_copy_kernel(const __grid_constant__ C
 // Products run on mma m16n8k16 (bf16, f32 sums) with the keys (or V's channels) as the 16
 // rows and 8 queries as the columns: the expanded cache is the A operand, which takes the
 // whole of a warp's lanes even for one query, is expanded once for all J query tiles, and
-// costs half the instructions of the form with queries as rows.  The kernel is bound by the
-// instructions that expand the numbers: a warp issues about 300 per 16 keys, half of them on
+// costs half the instructions of the form with queries as rows.  Among pages, the instructions
+// that expand the numbers are the limit: a warp issues about 300 per 16 keys, half of them on
 // the half-rate ALU pipe, and HBM rate would leave a scheduler 400 cycles for them.  With 16
 // warps per SM a page and head takes 0.28 us of an SM; HBM alone would take 0.21.  16 single
-// tokens over 1.3k to 10.6k keys, 32 heads: 97 us, 3.2 TB/s; one over 512 keys: 6 us.  (A
-// tcgen05 tile would need the expanded values written to shared memory again.)
+// tokens over 1.3k to 10.6k keys, 32 heads: 98 us, 3.2 TB/s.  The pages are 65 us of that; the
+// rest goes into uneven rows, the start of 4096 CTAs and their joins, so that over the call
+// nothing is near its limit (issue 52 %, ALU 44 %, HBM 38 %; the largest stalls are barriers
+// and fixed latencies).  One token over 512 keys: 6 us.  (A tcgen05 tile would need the
+// expanded values written to shared memory again.)
 //   S^T = K Q^T   K's values s * n are exact in bf16;
-//   O^T = V^T P^T V's too, P is rounded to bf16 as in the dense path; P^T comes out of S^T
-//                 by two 8x8 transposes (movmatrix).
+//   O^T = V^T P^T V's too.  P is rounded to bf16, the type of the product's operands, as in
+//                 the dense path (0.0021 off the 64-bit result in all where the output's own
+//                 rounding makes 0.0017; l sums P before the rounding, in f32); P^T comes out
+//                 of S^T by two 8x8 transposes (movmatrix).
 struct AttnParams4 {
   const uint8_t* pool;
   const int32_t* table;

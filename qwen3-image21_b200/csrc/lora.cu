@@ -16,9 +16,15 @@
 // C grows as the tiles get fewer, so that small calls still use the whole GPU; the loads of
 // step 3 start while step 2 runs.
 //
-// 4 requests of 4096 rows, 4096 -> 12288, rank 64: 177 us, 5.3 TB/s; step 1 runs at 4.8 TB/s,
-// step 2 takes 5 us, step 3 runs at 6.3 TB/s.  16 ragged requests of 4600 rows in all: 37 us,
-// of which 15 go into set-up, first loads and step 2.  4 single rows: 12.5 us, all latency.
+// u is rounded to bf16 because the second product's operands are bf16, as B is.  That is one
+// rounding more than the sums need (in all 0.0021 off the 64-bit result where the output's own
+// rounding makes 0.0017); the same product as two bf16 GEMMs rounds u in the same place.  Two
+// bf16 parts of u would avoid it for twice the second product and 16 or 32 KB of shared memory.
+//
+// On the GPU: 4 requests of 4096 rows, 4096 -> 12288, rank 64: 177 us, 5.3 TB/s (190 in a
+// series of calls on changing inputs); step 1 runs at 4.8 TB/s, step 2 takes 5 us, step 3 runs
+// at 6.3 TB/s.  16 ragged requests of 4600 rows in all: 37 us, of which 15 go into set-up,
+// first loads and step 2.  4 single rows: 12.9 us, all latency.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -742,9 +748,9 @@ extern "C" int b200_lora_add(const void* x, int64_t ldx, const void* a, const vo
   p.stage_bytes = kXBytes + regions * kTN * kTK * 2;
   const auto smem_of = [&](int stages) { return stages * p.stage_bytes + regions * kXBytes + kBarBytes + 1024; };
   // Every request ends in a tile of its own: rows / 128 + segments tiles at most.  The
-  // cluster is the largest whose tiles are expected to run all at once: with every request's
-  // last tile half full on average (16 ragged requests, 34 tiles: 72 us in clusters of 2, 43
-  // of 4, 37 of 6; of 8, 33 run at once and the 34th takes a second wave).
+  // cluster is the largest whose tiles are expected to run all at once, with every request's
+  // last tile half full on average.  (16 ragged requests of 4600 rows: 44 expected, and 44
+  // clusters of 6 run at once, 30 of 8; 72 us in clusters of 2, 43 of 4, 37 of 6.)
   const int64_t tiles = static_cast<int64_t>(rows) / kTM + std::min(segments, rows);
   const int64_t expect = std::min<int64_t>(tiles, (rows + kTM - 1) / kTM + segments / 2);
   const int steps = std::max((k + kTK - 1) / kTK, (n + kTN - 1) / kTN);
