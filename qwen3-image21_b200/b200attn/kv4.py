@@ -10,6 +10,7 @@ pages to the front of the pool.
 from __future__ import annotations
 
 import contextlib
+import copy
 import functools
 import heapq
 import threading
@@ -49,6 +50,13 @@ class PageTables:
         self._pages: Dict[int, List[int]] = {}
         self._length: Dict[int, int] = {}
         self._next = 0
+
+    def __getstate__(self):
+        with self.lock:  # copies and pickles carry the accounting, not the lock
+            return {k: copy.copy(v) for k, v in self.__dict__.items() if k != "lock"}
+
+    def __setstate__(self, state):
+        self.__dict__.update(state, lock=threading.RLock())
 
     @property
     def free_pages(self) -> int:

@@ -1,9 +1,11 @@
 """A 4-bit cache shared by host threads."""
+import copy
+import pickle
 import random
 import sys
 import threading
 
-from b200attn.kv4 import KV4Cache, OutOfPages
+from b200attn.kv4 import KV4Cache, OutOfPages, PageTables
 
 
 def test_threads_share_the_accounting():
@@ -46,3 +48,14 @@ def test_threads_share_the_accounting():
         sys.setswitchinterval(old)
     assert not failed, failed[:3]
     assert sorted(cache.tables._free) == list(range(40)) and not any(cache.tables._uses)
+
+
+def test_tables_can_be_copied_and_pickled():
+    """A copy plans ahead without touching the tables themselves."""
+    tables = PageTables(6)
+    a = tables.add(100)
+    for other in (copy.deepcopy(tables), pickle.loads(pickle.dumps(tables))):
+        other.extend([other.fork(a)], [70])
+        assert other.free_pages == 2 and other.pages(a) == [0, 1]
+        assert tables.free_pages == 4 and tables.pages(a) == [0, 1]
+        assert other.lock is not tables.lock
